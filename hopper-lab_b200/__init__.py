@@ -55,8 +55,15 @@ EXPORTS = [
     "b200_gemm_plan_create",
     "b200_gemm_plan_launch",
     "b200_gemm_plan_destroy",
+    "b200_mx_layout",
+    "b200_mx_quantize",
+    "b200_mx_dequantize",
+    "b200_mx_gemm",
+    "b200_mx_rms_norm",
 ]
 GATHER_MULTICAST, GATHER_PEERS = 1, 2
+MX_FORMATS = {"mxfp8": 0, "mxfp4": 1, "nvfp4": 2}
+MX_NORM_MAX_COLS = 32768
 
 
 class GemmArgs(C.Structure):
@@ -82,6 +89,39 @@ class GemmArgs(C.Structure):
         ("fault_inject", C.c_int32),
         ("wait_limit_ns", C.c_uint64),
         ("tile_n", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class MxDesc(C.Structure):
+    """Mirror of ``B200MxTensor`` (include/b200gemm.h)."""
+
+    _fields_ = [
+        ("format", C.c_int32),
+        ("reserved", C.c_int32),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("ld", C.c_int64),
+        ("data", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("tensor_scale", C.c_void_p),
+    ]
+
+
+class MxNormArgs(C.Structure):
+    """Mirror of ``B200MxNormArgs`` (include/b200gemm.h)."""
+
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("weight_dtype", C.c_int32),
+        ("x", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("h", C.c_void_p),
+        ("ldx", C.c_int64),
+        ("ldr", C.c_int64),
+        ("ldh", C.c_int64),
+        ("eps", C.c_float),
         ("reserved", C.c_int32),
     ]
 
@@ -131,6 +171,14 @@ def lib():
         L.b200_gemm_plan_launch.restype = C.c_int
         L.b200_gemm_plan_destroy.argtypes = [C.c_void_p]
         L.b200_gemm_plan_destroy.restype = None
+        L.b200_mx_layout.argtypes = [C.c_int32, C.c_int64, C.c_int64, C.POINTER(C.c_int64),
+                                     C.POINTER(C.c_int64)]
+        L.b200_mx_quantize.argtypes = [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32,
+                                       C.POINTER(MxDesc), C.c_void_p]
+        L.b200_mx_dequantize.argtypes = [C.POINTER(MxDesc), C.c_void_p, C.c_int32, C.c_int64, C.c_void_p]
+        L.b200_mx_gemm.argtypes = [C.POINTER(MxDesc), C.POINTER(MxDesc), C.c_void_p, C.c_int32, C.c_int64,
+                                   C.c_void_p]
+        L.b200_mx_rms_norm.argtypes = [C.POINTER(MxNormArgs), C.POINTER(MxDesc), C.c_void_p]
         _LIB = L
     return _LIB
 
@@ -340,3 +388,224 @@ def quantize_e4m3(x, q=None, scale=None, stream=None):
     if rc != OK:
         raise B200Error(rc, "b200_quantize_e4m3")
     return q, scale
+
+
+# ------------------------------------------------------------------ microscaled operands
+def mx_layout(fmt: str, rows: int, cols: int) -> tuple[int, int]:
+    """(bytes of one row of elements, bytes of all scale tiles) of a microscaled matrix."""
+    row, scale = C.c_int64(), C.c_int64()
+    rc = lib().b200_mx_layout(MX_FORMATS[fmt], rows, cols, C.byref(row), C.byref(scale))
+    if rc != OK:
+        raise B200Error(rc, "b200_mx_layout")
+    return row.value, scale.value
+
+
+class MxTensor:
+    """A microscaled matrix (``B200MxTensor``): 8- or 4-bit elements with a scale per block
+    of consecutive elements of a row.
+
+    ``fmt``           "mxfp8" (e4m3, blocks of 32), "mxfp4" (e2m1, blocks of 32) or "nvfp4"
+                      (e2m1, blocks of 16 with e4m3 scales and one fp32 scale)
+    ``rows, cols``    logical size; products sum over ``cols``
+    ``data``          uint8, rows x row bytes (cols padded to a multiple of 32 with zeros)
+    ``scales``        uint8, (ceil(rows / 128), tiles along the row, 32, 16), contiguous
+    ``tensor_scale``  1-element fp32 tensor or None ("nvfp4" only)
+    """
+
+    __slots__ = ("data", "scales", "fmt", "rows", "cols", "tensor_scale", "_desc", "_found")
+
+    def __init__(self, data, scales, fmt: str, rows: int, cols: int, tensor_scale=None):
+        torch = _torch()
+        row_bytes, scale_bytes = mx_layout(fmt, rows, cols)
+        if data.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("data and scales must be uint8 tensors")
+        if tuple(data.shape) != (rows, row_bytes) or (data.numel() > 0 and data.stride(1) != 1):
+            raise ValueError(f"data must be ({rows}, {row_bytes}) with unit column stride, not {tuple(data.shape)}")
+        if scales.numel() != scale_bytes or not scales.is_contiguous():
+            raise ValueError(f"scales must hold {scale_bytes} contiguous bytes, not {scales.numel()}")
+        if scales.device != data.device:
+            raise ValueError("data and scales must be on one device")
+        self.data, self.scales, self.fmt, self.rows, self.cols = data, scales, fmt, rows, cols
+        self._found = None
+        self._desc = None
+        self._set_scale(tensor_scale)
+
+    def _set_scale(self, tensor_scale):
+        torch = _torch()
+        if tensor_scale is not None:
+            if self.fmt != "nvfp4":
+                raise ValueError(f"{self.fmt} has no tensor scale")
+            if (tensor_scale.dtype != torch.float32 or tensor_scale.numel() != 1
+                    or tensor_scale.device != self.data.device):
+                raise ValueError("tensor_scale must be one float32 on the data's device")
+        if self._desc is not None and tensor_scale is self.tensor_scale:
+            return
+        self.tensor_scale = tensor_scale
+        self._desc = MxDesc(MX_FORMATS[self.fmt], 0, self.rows, self.cols,
+                            self.data.stride(0) if self.rows > 1 else self.data.shape[1], self.data.data_ptr(),
+                            self.scales.data_ptr(),
+                            self.tensor_scale.data_ptr() if self.tensor_scale is not None else None)
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, fmt: str, device="cuda", tensor_scale=None) -> "MxTensor":
+        """Uninitialised storage for a rows x cols matrix."""
+        torch = _torch()
+        row_bytes, scale_bytes = mx_layout(fmt, rows, cols)
+        bands = (rows + 127) // 128
+        data = torch.empty((rows, row_bytes), dtype=torch.uint8, device=device)
+        scales = torch.empty((bands, scale_bytes // 512 // max(bands, 1), 32, 16), dtype=torch.uint8, device=device)
+        return cls(data, scales, fmt, rows, cols, tensor_scale)
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.rows, self.cols
+
+    @property
+    def device(self):
+        return self.data.device
+
+
+def _mx_input(name, t):
+    """dtype code and row stride of a 2-D fp tensor with unit column stride."""
+    torch = _torch()
+    if t.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"{name} must be float16, bfloat16 or float32, not {t.dtype}")
+    if t.dim() != 2 or (t.numel() > 0 and t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be a 2-D row-major tensor with unit column stride")
+    return _dt_of(t), (t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1))
+
+
+def _mx_out(out, rows, cols, fmt, device, tensor_scale):
+    if fmt not in MX_FORMATS:
+        raise ValueError(f"unknown format {fmt!r}")
+    if out is None:
+        return MxTensor.empty(rows, cols, fmt, device, tensor_scale)
+    if out.fmt != fmt or out.shape != (rows, cols) or out.device != device:
+        raise ValueError(f"out is {out.fmt} {out.shape} on {out.device}, needed {fmt} {(rows, cols)} on {device}")
+    out._set_scale(tensor_scale)
+    return out
+
+
+class _On:
+    """Current device and stream of one call: what the call allocates belongs to the stream
+    that its kernels run on. ``stream``: None (the device's current one), a torch stream or a
+    raw handle."""
+
+    __slots__ = ("_device", "_stream", "handle")
+
+    def __init__(self, device, stream):
+        torch = _torch()
+        if device.type != "cuda":
+            raise ValueError(f"tensors must be on a CUDA device, not {device}")
+        self._device = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
+        self._stream = stream
+
+    def __enter__(self):
+        torch = _torch()
+        if self._device is not None:
+            self._device.__enter__()
+        if self._stream is None:
+            self.handle = torch.cuda.current_stream().cuda_stream
+        else:
+            if isinstance(self._stream, int):
+                self._stream = torch.cuda.ExternalStream(self._stream)
+            self.handle = self._stream.cuda_stream
+            self._stream = torch.cuda.stream(self._stream)
+            self._stream.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        if self._stream is not None:
+            self._stream.__exit__(*exc)
+        if self._device is not None:
+            self._device.__exit__(*exc)
+
+
+def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=None, out: MxTensor | None = None,
+                stream=None) -> MxTensor:
+    """Quantise a matrix (f16, bf16 or f32) to a microscaled one; with ``transpose`` its
+    transpose, for products that sum over x's rows. For "nvfp4", ``tensor_scale`` is one
+    positive fp32 on the device, used as given; None finds max|x| / 2688 in an extra pass.
+    ``out`` is written in place and takes the tensor scale."""
+    torch = _torch()
+    dt, ldx = _mx_input("x", x)
+    rows, cols = (x.shape[1], x.shape[0]) if transpose else (x.shape[0], x.shape[1])
+    with _On(x.device, stream) as on:
+        t = _mx_out(out, rows, cols, fmt, x.device, tensor_scale)
+        find = fmt == "nvfp4" and tensor_scale is None
+        if find:
+            if t._found is None:  # the scale and 12 bytes of scratch
+                t._found = torch.empty(4, dtype=torch.float32, device=x.device)
+            t._set_scale(t._found[:1])
+        rc = lib().b200_mx_quantize(x.data_ptr(), dt, ldx, int(transpose), int(find), C.byref(t._desc), on.handle)
+    if rc != OK:
+        raise B200Error(rc, "b200_mx_quantize")
+    return t
+
+
+def dequantize_mx(t: MxTensor, out=None, *, out_dtype="bf16", stream=None):
+    """The values a microscaled matrix stands for, rounded once to f16, bf16 or f32."""
+    torch = _torch()
+    with _On(t.device, stream) as on:
+        if out is None:
+            out = torch.empty((t.rows, t.cols), dtype=_torch_dtype(_dtype_code(out_dtype)), device=t.device)
+        dt, ldy = _mx_input("out", out)
+        if tuple(out.shape) != t.shape or out.device != t.device:
+            raise ValueError(f"out is {tuple(out.shape)} on {out.device}, needed {t.shape} on {t.device}")
+        rc = lib().b200_mx_dequantize(C.byref(t._desc), out.data_ptr(), dt, ldy, on.handle)
+    if rc != OK:
+        raise B200Error(rc, "b200_mx_dequantize")
+    return out
+
+
+def gemm_mx(a: MxTensor, b: MxTensor, c=None, *, out_dtype="bf16", stream=None):
+    """C = A . B^T of the values two microscaled matrices stand for (A: M x K, B: N x K,
+    same format), fp32 accumulation, to f16, bf16 or f32. Any row stride of C is accepted."""
+    torch = _torch()
+    if a.fmt != b.fmt:
+        raise TypeError(f"A and B must have the same format, not {a.fmt} and {b.fmt}")
+    if a.cols != b.cols or a.device != b.device:
+        raise ValueError(f"shape or device mismatch: A {a.shape} on {a.device}, B {b.shape} on {b.device}")
+    with _On(a.device, stream) as on:
+        if c is None:
+            c = torch.empty((a.rows, b.rows), dtype=_torch_dtype(_dtype_code(out_dtype)), device=a.device)
+        dt, ldc = _mx_input("C", c)
+        if tuple(c.shape) != (a.rows, b.rows) or c.device != a.device:
+            raise ValueError(f"C is {tuple(c.shape)} on {c.device}, needed {(a.rows, b.rows)} on {a.device}")
+        rc = lib().b200_mx_gemm(C.byref(a._desc), C.byref(b._desc), c.data_ptr(), dt, ldc, on.handle)
+    if rc != OK:
+        raise B200Error(rc, "b200_mx_gemm")
+    return c
+
+
+def rms_norm_mx(x, weight, residual=None, *, eps: float = 1e-6, fmt: str = "mxfp8", tensor_scale=None,
+                out: MxTensor | None = None, residual_out=None, stream=None):
+    """RMS norm with the residual's addition, to a microscaled matrix: h = x + residual,
+    out = quantised(h / sqrt(mean(h^2) + eps) * weight). Returns (out, h), h rounded to x's
+    type, or (out, None) without a residual. ``residual_out`` may be ``residual`` or ``x``.
+    ``weight`` has x's type or is float32; ``tensor_scale`` ("nvfp4") is used as given, None
+    stands for 1, which suits normalised rows (block maxima from 0.006 to 2688)."""
+    torch = _torch()
+    dt, ldx = _mx_input("x", x)
+    rows, cols = x.shape
+    if weight.dim() != 1 or weight.shape[0] != cols or not weight.is_contiguous() or weight.device != x.device:
+        raise ValueError(f"weight must hold {cols} contiguous elements on {x.device}")
+    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+        raise TypeError(f"weight must be {x.dtype} or float32, not {weight.dtype}")
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    with _On(x.device, stream) as on:
+        args = MxNormArgs(dt, _dt_of(weight), x.data_ptr(), weight.data_ptr(), None, None, ldx, 0, 0, eps, 0)
+        if residual is not None:
+            if residual_out is None:
+                residual_out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+            for name, t in (("residual", residual), ("residual_out", residual_out)):
+                if t.dtype != x.dtype or t.shape != x.shape or t.device != x.device:
+                    raise ValueError(f"{name} must match x: {x.dtype} {tuple(x.shape)} on {x.device}")
+            args.residual, args.h = residual.data_ptr(), residual_out.data_ptr()
+            args.ldr, args.ldh = _mx_input("residual", residual)[1], _mx_input("residual_out", residual_out)[1]
+        t = _mx_out(out, rows, cols, fmt, x.device, tensor_scale)
+        rc = lib().b200_mx_rms_norm(C.byref(args), C.byref(t._desc), on.handle)
+    if rc != OK:
+        raise B200Error(rc, "b200_mx_rms_norm")
+    return t, residual_out

@@ -752,6 +752,22 @@ namespace b200 {
 
 int gemm_validate(const B200GemmArgs* a) { return validate(a); }
 
+int gemm_device(int* dev, int* sms, uint32_t** status) {
+  int d = 0;
+  int rc = device_setup(&d);
+  if (rc != B200_OK) return rc;
+  if (g_cc_major[d] != 10) return B200_ERR_UNSUPPORTED;
+  if (dev) *dev = d;
+  if (sms) *sms = g_sm_count[d];
+  if (status) *status = status_word(d);
+  return B200_OK;
+}
+
+int gemm_encode_2d(CUtensorMap* m, const void* ptr, int dt, uint64_t rows, uint64_t cols, uint64_t ld,
+                   uint32_t box_rows, uint32_t box_cols) {
+  return encode_2d(m, ptr, dt, rows, cols, ld, box_rows, box_cols);
+}
+
 int gemm_resolve_driver() {
   std::lock_guard<std::mutex> lk(g_mu);
   return resolve_encode();

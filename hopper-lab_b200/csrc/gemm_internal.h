@@ -50,6 +50,18 @@ struct Prepared {
   size_t c_pitch, c_width, c_height;
 };
 
+// Set up the current device once and report it: its index, SM count and status word
+// (any may be null). B200_ERR_UNSUPPORTED when it is not sm_100.
+int gemm_device(int* dev, int* sms, uint32_t** status);
+
+// Tensor map of a row-major [rows x cols] matrix, box [box_rows x box_cols], 128-byte
+// swizzle; gemm_device() must have succeeded.
+int gemm_encode_2d(CUtensorMap* m, const void* ptr, int dt, uint64_t rows, uint64_t cols, uint64_t ld,
+                   uint32_t box_rows, uint32_t box_cols);
+
+// Checks of one microscaled operand that need no GPU.
+int mx_validate(const B200MxTensor* t);
+
 int gemm_prepare(const B200GemmArgs& a, int sms, int cc_major, uint32_t* status, bool allow_workspace,
                  const GatherSpec* gather, Prepared* out);
 int gemm_launch_prepared(Prepared& pr, cudaStream_t stream);

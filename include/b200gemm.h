@@ -197,6 +197,84 @@ int b200_gemm_allgather(const B200GemmArgs* args, const void* dst, int32_t mode,
  * without a scale. Stream-ordered; returns B200_OK or a negative code. */
 int b200_quantize_e4m3(const float* x, int64_t n, void* q, float* scale, void* stream);
 
+/* ---- microscaled operands ------------------------------------------------------
+ * A microscaled matrix holds `rows` rows of 8- or 4-bit elements and one scale per block
+ * of consecutive elements of a row, with the blocks along the dimension a product sums
+ * over:
+ *   B200_MX_FP8  e4m3 elements, blocks of 32, scale 2^(byte - 127) (e8m0; 0xFF = NaN)
+ *   B200_MX_FP4  e2m1 elements, blocks of 32, scale 2^(byte - 127)
+ *   B200_NV_FP4  e2m1 elements, blocks of 16, scale e4m3, and one fp32 scale for the
+ *                whole matrix
+ * element i of row r stands for element * block scale * tensor scale.
+ *   data    row r starts at byte r * ld; a row holds ceil(cols / 32) * 32 elements (the
+ *           ones behind `cols` are zero), two 4-bit elements to a byte, the first in the
+ *           low half
+ *   scales  tiles of 128 rows x 4 blocks, 512 bytes: row r, block c of a tile is byte
+ *           (r % 32) * 16 + (r / 32) * 4 + c; the tiles of a 128-row band follow one
+ *           another along the row, the bands one another; padding bytes are zero
+ * b200_mx_layout gives both sizes. Data, scales and ld are 16-byte aligned. */
+enum { B200_MX_FP8 = 0, B200_MX_FP4 = 1, B200_NV_FP4 = 2 };
+
+typedef struct B200MxTensor {
+  int32_t format;      /* B200_MX_FP8 | B200_MX_FP4 | B200_NV_FP4                        */
+  int32_t reserved;    /* must be 0                                                      */
+  int64_t rows, cols;  /* logical size; both below 2^31 - 128                            */
+  int64_t ld;          /* bytes between rows of data: >= row_bytes, a multiple of 16     */
+  void* data;
+  void* scales;
+  float* tensor_scale; /* B200_NV_FP4: device fp32 scalar or NULL (1.0); else NULL       */
+} B200MxTensor;
+
+/* Bytes of one row of data and of all scale tiles. Needs no GPU. */
+int b200_mx_layout(int32_t format, int64_t rows, int64_t cols, int64_t* row_bytes, int64_t* scale_bytes);
+
+/* Quantise x into q (its padding included). x_dtype: B200_DT_F16 | B200_DT_BF16 |
+ * B200_DT_F32; ldx: elements between x's rows. transpose = 0: x is q->rows x q->cols and
+ * blocks run along its rows; transpose != 0: x is q->cols x q->rows and q holds its
+ * transpose, for products that sum over x's rows.
+ *   MX formats: a block's scale is the smallest 2^e, e >= -127, with amax <= max * 2^e
+ *     (max 448 or 6), so no element saturates; element = nearest(x / 2^e).
+ *   B200_NV_FP4: u = x * fl32(1 / tensor scale), rounded to fp32; block scale =
+ *     nearest_e4m3(min(max|u| / 6, 448)); element = nearest_e2m1(u / block scale),
+ *     saturating at 6; all elements are 0 where the scale rounds to 0.
+ * Ties go to the even significand. A block that holds a NaN or an infinity (or a u that
+ * is not finite) gets a NaN scale and makes every sum it enters NaN.
+ * find_scale != 0 (B200_NV_FP4): the tensor scale is max|x| / 2688 over the finite
+ * elements (at least 2^-126; 1 when all are 0), written to q->tensor_scale, which then
+ * points to 16 writable bytes, 16-byte aligned (the other 12 are scratch). Otherwise the
+ * scale at q->tensor_scale is used as given: positive and normal. */
+int b200_mx_quantize(const void* x, int32_t x_dtype, int64_t ldx, int32_t transpose, int32_t find_scale,
+                     const B200MxTensor* q, void* stream);
+
+/* y (q->rows x q->cols, f16 / bf16 / f32, ldy elements between rows) = the values q
+ * stands for, rounded once. */
+int b200_mx_dequantize(const B200MxTensor* q, void* y, int32_t y_dtype, int64_t ldy, void* stream);
+
+/* C (a->rows x b->rows) = A . B^T of the values two microscaled matrices of the same
+ * format and `cols` stand for, fp32 accumulation, one rounding to c_dtype (B200_DT_F16 |
+ * B200_DT_BF16 | B200_DT_F32). ldc >= b->rows elements; C is aligned to its element and
+ * any ldc is accepted. Waits are bounded as b200_gemm's (b200_gemm_status). */
+int b200_mx_gemm(const B200MxTensor* a, const B200MxTensor* b, void* c, int32_t c_dtype, int64_t ldc,
+                 void* stream);
+
+/* RMS norm to a microscaled matrix: for each row, h = x + residual (x alone without a
+ * residual), y = h / sqrt(mean(h^2) + eps) * weight in fp32, q = quantised y (the tensor
+ * scale of a B200_NV_FP4 q is used as given). With a residual, h is also stored, rounded
+ * to dtype; h may be the same memory as x or residual. cols <= B200_MX_NORM_MAX_COLS. */
+#define B200_MX_NORM_MAX_COLS 32768
+typedef struct B200MxNormArgs {
+  int32_t dtype;        /* of x, residual and h: B200_DT_F16 | B200_DT_BF16 | B200_DT_F32 */
+  int32_t weight_dtype; /* dtype or B200_DT_F32                                           */
+  const void* x;
+  const void* weight;   /* cols elements                                                  */
+  const void* residual; /* or NULL                                                        */
+  void* h;              /* needed with a residual, ignored without                        */
+  int64_t ldx, ldr, ldh; /* elements between rows, >= cols                                */
+  float eps;            /* >= 0                                                           */
+  int32_t reserved;     /* must be 0                                                      */
+} B200MxNormArgs;
+int b200_mx_rms_norm(const B200MxNormArgs* args, const B200MxTensor* q, void* stream);
+
 /* ABI version (B200GEMM_ABI_VERSION). */
 int b200_gemm_abi_version(void);
 
