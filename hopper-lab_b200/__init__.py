@@ -391,6 +391,11 @@ def quantize_e4m3(x, q=None, scale=None, stream=None):
 
 
 # ------------------------------------------------------------------ microscaled operands
+# These calls are short kernels, so their host side is kept short too: one allocation for a
+# microscaled matrix, views of it only when asked for, raw stream handles.
+_MX_BLOCK = {"mxfp8": 32, "mxfp4": 32, "nvfp4": 16}
+
+
 def mx_layout(fmt: str, rows: int, cols: int) -> tuple[int, int]:
     """(bytes of one row of elements, bytes of all scale tiles) of a microscaled matrix."""
     row, scale = C.c_int64(), C.c_int64()
@@ -412,7 +417,7 @@ class MxTensor:
     ``tensor_scale``  1-element fp32 tensor or None ("nvfp4" only)
     """
 
-    __slots__ = ("data", "scales", "fmt", "rows", "cols", "tensor_scale", "_desc", "_found")
+    __slots__ = ("_data", "_scales", "fmt", "rows", "cols", "device", "_ts", "_desc", "_ref", "_own", "_off")
 
     def __init__(self, data, scales, fmt: str, rows: int, cols: int, tensor_scale=None):
         torch = _torch()
@@ -425,91 +430,144 @@ class MxTensor:
             raise ValueError(f"scales must hold {scale_bytes} contiguous bytes, not {scales.numel()}")
         if scales.device != data.device:
             raise ValueError("data and scales must be on one device")
-        self.data, self.scales, self.fmt, self.rows, self.cols = data, scales, fmt, rows, cols
-        self._found = None
-        self._desc = None
-        self._set_scale(tensor_scale)
-
-    def _set_scale(self, tensor_scale):
-        torch = _torch()
-        if tensor_scale is not None:
-            if self.fmt != "nvfp4":
-                raise ValueError(f"{self.fmt} has no tensor scale")
-            if (tensor_scale.dtype != torch.float32 or tensor_scale.numel() != 1
-                    or tensor_scale.device != self.data.device):
-                raise ValueError("tensor_scale must be one float32 on the data's device")
-        if self._desc is not None and tensor_scale is self.tensor_scale:
-            return
+        self._data, self._scales, self._own, self._off, self._ts = data, scales, None, 0, None
+        self.fmt, self.rows, self.cols, self.device = fmt, rows, cols, data.device
+        self._desc = MxDesc(MX_FORMATS[fmt], 0, rows, cols, data.stride(0) if rows > 1 else row_bytes,
+                            data.data_ptr(), scales.data_ptr(), None)
+        self._ref = C.byref(self._desc)
         self.tensor_scale = tensor_scale
-        self._desc = MxDesc(MX_FORMATS[self.fmt], 0, self.rows, self.cols,
-                            self.data.stride(0) if self.rows > 1 else self.data.shape[1], self.data.data_ptr(),
-                            self.scales.data_ptr(),
-                            self.tensor_scale.data_ptr() if self.tensor_scale is not None else None)
 
     @classmethod
     def empty(cls, rows: int, cols: int, fmt: str, device="cuda", tensor_scale=None) -> "MxTensor":
         """Uninitialised storage for a rows x cols matrix."""
+        mx_layout(fmt, rows, cols)  # refuses what has no layout
+        t = cls._new(rows, cols, fmt, device)
+        if tensor_scale is not None:
+            t.tensor_scale = tensor_scale
+        return t
+
+    @classmethod
+    def _new(cls, rows, cols, fmt, device):
+        # one buffer: scale tiles, 256 bytes with a tensor scale and its scratch, element rows
+        blk = _MX_BLOCK[fmt]
+        kp = (cols + 31) // 32 * 32
+        scale_bytes = (rows + 127) // 128 * ((kp // blk + 3) // 4) * 512
+        row_bytes = kp if fmt == "mxfp8" else kp // 2
+        self = object.__new__(cls)
         torch = _torch()
-        row_bytes, scale_bytes = mx_layout(fmt, rows, cols)
-        bands = (rows + 127) // 128
-        data = torch.empty((rows, row_bytes), dtype=torch.uint8, device=device)
-        scales = torch.empty((bands, scale_bytes // 512 // max(bands, 1), 32, 16), dtype=torch.uint8, device=device)
-        return cls(data, scales, fmt, rows, cols, tensor_scale)
+        self._own = buf = torch.empty(scale_bytes + 256 + rows * row_bytes, dtype=torch.uint8, device=device)
+        self._off = scale_bytes
+        ptr = buf.data_ptr()
+        self._data = self._scales = self._ts = None
+        self.fmt, self.rows, self.cols, self.device = fmt, rows, cols, buf.device
+        self._desc = MxDesc(MX_FORMATS[fmt], 0, rows, cols, row_bytes, ptr + scale_bytes + 256, ptr, None)
+        self._ref = C.byref(self._desc)
+        return self
+
+    @property
+    def data(self):
+        if self._data is None:
+            ld = self._desc.ld
+            self._data = self._own.as_strided((self.rows, ld), (ld, 1), self._off + 256)
+        return self._data
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            bands = (self.rows + 127) // 128
+            tiles = self._off // 512 // max(bands, 1)
+            self._scales = self._own.as_strided((bands, tiles, 32, 16), (tiles * 512, 512, 16, 1), 0)
+        return self._scales
+
+    @property
+    def tensor_scale(self):
+        if self._ts is None and self._desc.tensor_scale is not None:
+            # found by the quantiser into this matrix's own buffer
+            self._ts = self._own[self._off:self._off + 4].view(_torch().float32)
+        return self._ts
+
+    @tensor_scale.setter
+    def tensor_scale(self, ts):
+        if ts is not None:
+            if self.fmt != "nvfp4":
+                raise ValueError(f"{self.fmt} has no tensor scale")
+            if ts.dtype != _torch().float32 or ts.numel() != 1 or ts.device != self.device:
+                raise ValueError("tensor_scale must be one float32 on the data's device")
+        self._ts = ts
+        self._desc.tensor_scale = None if ts is None else ts.data_ptr()
+
+    def _scratch(self):
+        """16 bytes for a tensor scale to be found into."""
+        if self._own is None:  # data and scales are the caller's: a buffer beside them
+            self._own = _torch().empty(256, dtype=_torch().uint8, device=self.device)
+        self._ts = None
+        self._desc.tensor_scale = self._own.data_ptr() + self._off
 
     @property
     def shape(self) -> tuple[int, int]:
         return self.rows, self.cols
 
-    @property
-    def device(self):
-        return self.data.device
+
+_MX_IN = {}
 
 
 def _mx_input(name, t):
     """dtype code and row stride of a 2-D fp tensor with unit column stride."""
-    torch = _torch()
-    if t.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+    if not _MX_IN:
+        torch = _torch()
+        _MX_IN.update({torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: DT_F32})
+    dt = _MX_IN.get(t.dtype)
+    if dt is None:
         raise TypeError(f"{name} must be float16, bfloat16 or float32, not {t.dtype}")
-    if t.dim() != 2 or (t.numel() > 0 and t.shape[1] > 1 and t.stride(1) != 1):
+    shape = t.shape
+    if len(shape) != 2:
         raise ValueError(f"{name} must be a 2-D row-major tensor with unit column stride")
-    return _dt_of(t), (t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1))
+    ld, unit = t.stride()
+    if unit != 1 and shape[1] > 1 and shape[0] > 0:
+        raise ValueError(f"{name} must be a 2-D row-major tensor with unit column stride")
+    return dt, ld if shape[0] > 1 else max(shape[1], 1)
+
+
+_MX_OUT = {}
+
+
+def _mx_out_dtype(name):
+    dt = _MX_OUT.get(name)
+    if dt is None:
+        dt = _MX_OUT[name] = _torch_dtype(_dtype_code(name))
+    return dt
 
 
 def _mx_out(out, rows, cols, fmt, device, tensor_scale):
     if fmt not in MX_FORMATS:
         raise ValueError(f"unknown format {fmt!r}")
     if out is None:
-        return MxTensor.empty(rows, cols, fmt, device, tensor_scale)
-    if out.fmt != fmt or out.shape != (rows, cols) or out.device != device:
+        out = MxTensor._new(rows, cols, fmt, device)
+        if tensor_scale is not None:
+            out.tensor_scale = tensor_scale
+        return out
+    if out.fmt != fmt or out.rows != rows or out.cols != cols or out.device != device:
         raise ValueError(f"out is {out.fmt} {out.shape} on {out.device}, needed {fmt} {(rows, cols)} on {device}")
-    out._set_scale(tensor_scale)
+    out.tensor_scale = tensor_scale
     return out
 
 
 class _On:
     """Current device and stream of one call: what the call allocates belongs to the stream
-    that its kernels run on. ``stream``: None (the device's current one), a torch stream or a
-    raw handle."""
+    that its kernels run on. ``stream``: a torch stream or a raw handle."""
 
     __slots__ = ("_device", "_stream", "handle")
 
     def __init__(self, device, stream):
         torch = _torch()
-        if device.type != "cuda":
-            raise ValueError(f"tensors must be on a CUDA device, not {device}")
-        self._device = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
-        self._stream = stream
+        self._device = torch.cuda.device(device)
+        self._stream = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
 
     def __enter__(self):
         torch = _torch()
-        if self._device is not None:
-            self._device.__enter__()
-        if self._stream is None:
-            self.handle = torch.cuda.current_stream().cuda_stream
-        else:
-            if isinstance(self._stream, int):
-                self._stream = torch.cuda.ExternalStream(self._stream)
-            self.handle = self._stream.cuda_stream
+        self._device.__enter__()
+        self.handle = (self._stream or torch.cuda.current_stream()).cuda_stream
+        if self._stream is not None:
             self._stream = torch.cuda.stream(self._stream)
             self._stream.__enter__()
         return self
@@ -517,8 +575,30 @@ class _On:
     def __exit__(self, *exc):
         if self._stream is not None:
             self._stream.__exit__(*exc)
-        if self._device is not None:
-            self._device.__exit__(*exc)
+        self._device.__exit__(*exc)
+
+
+class _Here:
+    """_On for the usual call: the current device and its current stream."""
+
+    __slots__ = ("handle",)
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        pass
+
+
+def _on(device, stream):
+    if device.type != "cuda":
+        raise ValueError(f"tensors must be on a CUDA device, not {device}")
+    cuda = _torch().cuda
+    if stream is None and cuda.current_device() == device.index:
+        here = _Here()
+        here.handle = _torch()._C._cuda_getCurrentRawStream(device.index)
+        return here
+    return _On(device, stream)
 
 
 def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=None, out: MxTensor | None = None,
@@ -527,17 +607,17 @@ def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=
     transpose, for products that sum over x's rows. For "nvfp4", ``tensor_scale`` is one
     positive fp32 on the device, used as given; None finds max|x| / 2688 in an extra pass.
     ``out`` is written in place and takes the tensor scale."""
-    torch = _torch()
     dt, ldx = _mx_input("x", x)
-    rows, cols = (x.shape[1], x.shape[0]) if transpose else (x.shape[0], x.shape[1])
-    with _On(x.device, stream) as on:
-        t = _mx_out(out, rows, cols, fmt, x.device, tensor_scale)
+    rows, cols = x.shape
+    if transpose:
+        rows, cols = cols, rows
+    device = x.device
+    with _on(device, stream) as on:
+        t = _mx_out(out, rows, cols, fmt, device, tensor_scale)
         find = fmt == "nvfp4" and tensor_scale is None
         if find:
-            if t._found is None:  # the scale and 12 bytes of scratch
-                t._found = torch.empty(4, dtype=torch.float32, device=x.device)
-            t._set_scale(t._found[:1])
-        rc = lib().b200_mx_quantize(x.data_ptr(), dt, ldx, int(transpose), int(find), C.byref(t._desc), on.handle)
+            t._scratch()
+        rc = (_LIB or lib()).b200_mx_quantize(x.data_ptr(), dt, ldx, transpose, find, t._ref, on.handle)
     if rc != OK:
         raise B200Error(rc, "b200_mx_quantize")
     return t
@@ -545,14 +625,14 @@ def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=
 
 def dequantize_mx(t: MxTensor, out=None, *, out_dtype="bf16", stream=None):
     """The values a microscaled matrix stands for, rounded once to f16, bf16 or f32."""
-    torch = _torch()
-    with _On(t.device, stream) as on:
+    device = t.device
+    with _on(device, stream) as on:
         if out is None:
-            out = torch.empty((t.rows, t.cols), dtype=_torch_dtype(_dtype_code(out_dtype)), device=t.device)
+            out = _torch().empty((t.rows, t.cols), dtype=_mx_out_dtype(out_dtype), device=device)
+        elif tuple(out.shape) != t.shape or out.device != device:
+            raise ValueError(f"out is {tuple(out.shape)} on {out.device}, needed {t.shape} on {device}")
         dt, ldy = _mx_input("out", out)
-        if tuple(out.shape) != t.shape or out.device != t.device:
-            raise ValueError(f"out is {tuple(out.shape)} on {out.device}, needed {t.shape} on {t.device}")
-        rc = lib().b200_mx_dequantize(C.byref(t._desc), out.data_ptr(), dt, ldy, on.handle)
+        rc = (_LIB or lib()).b200_mx_dequantize(t._ref, out.data_ptr(), dt, ldy, on.handle)
     if rc != OK:
         raise B200Error(rc, "b200_mx_dequantize")
     return out
@@ -561,18 +641,18 @@ def dequantize_mx(t: MxTensor, out=None, *, out_dtype="bf16", stream=None):
 def gemm_mx(a: MxTensor, b: MxTensor, c=None, *, out_dtype="bf16", stream=None):
     """C = A . B^T of the values two microscaled matrices stand for (A: M x K, B: N x K,
     same format), fp32 accumulation, to f16, bf16 or f32. Any row stride of C is accepted."""
-    torch = _torch()
+    device = a.device
     if a.fmt != b.fmt:
         raise TypeError(f"A and B must have the same format, not {a.fmt} and {b.fmt}")
-    if a.cols != b.cols or a.device != b.device:
-        raise ValueError(f"shape or device mismatch: A {a.shape} on {a.device}, B {b.shape} on {b.device}")
-    with _On(a.device, stream) as on:
+    if a.cols != b.cols or device != b.device:
+        raise ValueError(f"shape or device mismatch: A {a.shape} on {device}, B {b.shape} on {b.device}")
+    with _on(device, stream) as on:
         if c is None:
-            c = torch.empty((a.rows, b.rows), dtype=_torch_dtype(_dtype_code(out_dtype)), device=a.device)
+            c = _torch().empty((a.rows, b.rows), dtype=_mx_out_dtype(out_dtype), device=device)
+        elif tuple(c.shape) != (a.rows, b.rows) or c.device != device:
+            raise ValueError(f"C is {tuple(c.shape)} on {c.device}, needed {(a.rows, b.rows)} on {device}")
         dt, ldc = _mx_input("C", c)
-        if tuple(c.shape) != (a.rows, b.rows) or c.device != a.device:
-            raise ValueError(f"C is {tuple(c.shape)} on {c.device}, needed {(a.rows, b.rows)} on {a.device}")
-        rc = lib().b200_mx_gemm(C.byref(a._desc), C.byref(b._desc), c.data_ptr(), dt, ldc, on.handle)
+        rc = (_LIB or lib()).b200_mx_gemm(a._ref, b._ref, c.data_ptr(), dt, ldc, on.handle)
     if rc != OK:
         raise B200Error(rc, "b200_mx_gemm")
     return c
@@ -585,27 +665,34 @@ def rms_norm_mx(x, weight, residual=None, *, eps: float = 1e-6, fmt: str = "mxfp
     type, or (out, None) without a residual. ``residual_out`` may be ``residual`` or ``x``.
     ``weight`` has x's type or is float32; ``tensor_scale`` ("nvfp4") is used as given, None
     stands for 1, which suits normalised rows (block maxima from 0.006 to 2688)."""
-    torch = _torch()
     dt, ldx = _mx_input("x", x)
-    rows, cols = x.shape
-    if weight.dim() != 1 or weight.shape[0] != cols or not weight.is_contiguous() or weight.device != x.device:
-        raise ValueError(f"weight must hold {cols} contiguous elements on {x.device}")
-    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+    rows, cols = shape = x.shape
+    device = x.device
+    wt = _MX_IN.get(weight.dtype)
+    if weight.shape != (cols,) or not weight.is_contiguous() or weight.device != device:
+        raise ValueError(f"weight must hold {cols} contiguous elements on {device}")
+    if wt != dt and wt != DT_F32:
         raise TypeError(f"weight must be {x.dtype} or float32, not {weight.dtype}")
     if residual is None and residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    with _On(x.device, stream) as on:
-        args = MxNormArgs(dt, _dt_of(weight), x.data_ptr(), weight.data_ptr(), None, None, ldx, 0, 0, eps, 0)
-        if residual is not None:
+    with _on(device, stream) as on:
+        if residual is None:
+            args = MxNormArgs(dt, wt, x.data_ptr(), weight.data_ptr(), None, None, ldx, 0, 0, eps, 0)
+        else:
             if residual_out is None:
-                residual_out = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-            for name, t in (("residual", residual), ("residual_out", residual_out)):
-                if t.dtype != x.dtype or t.shape != x.shape or t.device != x.device:
-                    raise ValueError(f"{name} must match x: {x.dtype} {tuple(x.shape)} on {x.device}")
-            args.residual, args.h = residual.data_ptr(), residual_out.data_ptr()
-            args.ldr, args.ldh = _mx_input("residual", residual)[1], _mx_input("residual_out", residual_out)[1]
-        t = _mx_out(out, rows, cols, fmt, x.device, tensor_scale)
-        rc = lib().b200_mx_rms_norm(C.byref(args), C.byref(t._desc), on.handle)
+                residual_out = _torch().empty((rows, cols), dtype=x.dtype, device=device)
+            elif residual_out.shape != shape or residual_out.device != device:
+                raise ValueError(f"residual_out must match x: {tuple(shape)} on {device}")
+            if residual.shape != shape or residual.device != device:
+                raise ValueError(f"residual must match x: {tuple(shape)} on {device}")
+            rt, ldr = _mx_input("residual", residual)
+            ht, ldh = _mx_input("residual_out", residual_out)
+            if rt != dt or ht != dt:
+                raise TypeError(f"residual and residual_out must be {x.dtype}")
+            args = MxNormArgs(dt, wt, x.data_ptr(), weight.data_ptr(), residual.data_ptr(), residual_out.data_ptr(),
+                              ldx, ldr, ldh, eps, 0)
+        t = _mx_out(out, rows, cols, fmt, device, tensor_scale)
+        rc = (_LIB or lib()).b200_mx_rms_norm(C.byref(args), t._ref, on.handle)
     if rc != OK:
         raise B200Error(rc, "b200_mx_rms_norm")
     return t, residual_out

@@ -768,6 +768,19 @@ int gemm_encode_2d(CUtensorMap* m, const void* ptr, int dt, uint64_t rows, uint6
   return encode_2d(m, ptr, dt, rows, cols, ld, box_rows, box_cols);
 }
 
+int gemm_encode_tiles(CUtensorMap* m, const void* ptr, uint64_t groups, uint64_t bands, uint32_t groups_box,
+                      uint32_t bands_box) {
+  const cuuint64_t gdim[3] = {128, groups, bands};
+  const cuuint64_t gstride[2] = {512, groups * 512};
+  const cuuint32_t box[3] = {128, groups_box, bands_box};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  std::memset(m, 0, sizeof(*m));
+  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(ptr), gdim, gstride, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200_OK : B200_ERR_TMAP;
+}
+
 int gemm_resolve_driver() {
   std::lock_guard<std::mutex> lk(g_mu);
   return resolve_encode();

@@ -59,6 +59,11 @@ int gemm_device(int* dev, int* sms, uint32_t** status);
 int gemm_encode_2d(CUtensorMap* m, const void* ptr, int dt, uint64_t rows, uint64_t cols, uint64_t ld,
                    uint32_t box_rows, uint32_t box_cols);
 
+// Tensor map of `bands` x `groups` contiguous 512-byte tiles, box bands_box x groups_box
+// tiles, no swizzle.
+int gemm_encode_tiles(CUtensorMap* m, const void* ptr, uint64_t groups, uint64_t bands, uint32_t groups_box,
+                      uint32_t bands_box);
+
 // Checks of one microscaled operand that need no GPU.
 int mx_validate(const B200MxTensor* t);
 

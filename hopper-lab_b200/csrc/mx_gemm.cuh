@@ -92,6 +92,16 @@ __device__ __forceinline__ float4 ld_shared_cluster_f4(uint32_t addr) {
   return v;
 }
 
+// True in one lane of the (converged) warp. The compiler knows a branch on elect.sync to
+// be taken by one thread, so descriptors and addresses inside it go straight to uniform
+// registers; under `lane == 0` every MMA or scale copy pays a per-lane loop instead:
+// 119 clocks per MMA and 14 per copy measured, against 96 (N = 192, copies hidden).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---------------------------------------------------------------------------------
 // format facts of one 128-byte K atom
 // ---------------------------------------------------------------------------------
@@ -102,6 +112,39 @@ struct MxAtom {
   // first scale in the tile's 4-byte words
   static constexpr uint32_t group(uint32_t s) { return FMT == MX_FP8 ? 0 : FMT == MX_FP4 ? s / 2 : s; }
   static constexpr uint32_t sf_id(uint32_t s) { return FMT == MX_FP8 ? s : FMT == MX_FP4 ? 2 * (s % 2) : 0; }
+};
+
+// Scale copies and MMAs of one stage, issued by one thread: `g_n` scale tiles per band,
+// `steps` MMA steps, both at their maximum when FULL. The issue itself is what a stage can
+// wait for (16 copies and 8 MMAs against 768 clocks of MMA time), so a full stage has no
+// run-time conditions, and every descriptor is a base plus a constant: with a condition per
+// step a 192-wide pair stage took 511 clocks, without 386 (its MMAs alone: 384).
+//   sa / sb     TMEM columns of the two operands' scales; BANDS tiles of 4 columns per group
+//   a / b       shared-memory descriptors of the first step
+//   d           first accumulator column
+template <int CG, int FMT, uint32_t N, uint32_t BANDS, bool FULL>
+struct MxStage {
+  using Atom = MxAtom<FMT>;
+  static __device__ __forceinline__ void copy_scales(uint32_t sa, uint32_t sb, uint64_t tile_a, uint64_t tile_b,
+                                                     uint32_t g_n) {
+#pragma unroll
+    for (uint32_t g = 0; g < Atom::GROUPS; ++g) {
+      if (FULL || g < g_n) {
+        tmem_cp_scales<CG>(sa + 4 * g, tile_a + g * 32u);
+#pragma unroll
+        for (uint32_t b = 0; b < BANDS; ++b)
+          tmem_cp_scales<CG>(sb + 4 * (BANDS * g + b), tile_b + (b * Atom::GROUPS + g) * 32u);
+      }
+    }
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t sa, uint32_t sb,
+                                             uint32_t steps, uint32_t accumulate) {
+#pragma unroll
+    for (uint32_t s = 0; s < 4; ++s)
+      if (FULL || s < steps)
+        umma_mx<CG, FMT>(d, a + 2 * s, b + 2 * s, idesc_mx<FMT>(128 * CG, N, Atom::sf_id(s)), sa + 4 * Atom::group(s),
+                         sb + 4 * BANDS * Atom::group(s), s ? 1u : accumulate);
+  }
 };
 
 struct MxParams {
@@ -127,29 +170,31 @@ struct MxParams {
 // ---------------------------------------------------------------------------------
 // The accumulator is C transposed: TMEM lane = row of B (column of C), column = row of A.
 // With few rows of A the weights B are the long operand and take the MMA's 128-row side;
-// the other side is only as wide as the tokens need (NT = 16 ... 256), so one token does
+// the other side is only as wide as the tokens need (NT = 16 ... 128), so one token does
 // not pay for 128. K is split over a cluster of up to 8 CTAs when the tiles alone leave
 // SMs idle; the partial sums meet in distributed shared memory, added in rank order, so
 // results do not depend on timing and no workspace or second launch is needed.
 template <int FMT, int NT>
 struct MxRowsCfg {
   static constexpr uint32_t GROUPS = MxAtom<FMT>::GROUPS;
-  static constexpr uint32_t QB = NT > 128 ? NT / 128 : 1;  // scale bands of Q
   static constexpr uint32_t P_BYTES = 128 * 128;
   static constexpr uint32_t Q_BYTES = NT * 128;
   static constexpr uint32_t SFP_BYTES = GROUPS * 512;
-  static constexpr uint32_t SFQ_BYTES = QB * GROUPS * 512;
+  static constexpr uint32_t SFQ_BYTES = GROUPS * 512;
   static constexpr uint32_t STAGE = P_BYTES + Q_BYTES + SFP_BYTES + SFQ_BYTES;
   static constexpr uint32_t BAR_BYTES = 256;
   static constexpr uint32_t MAX_SMEM = 232448;
   static constexpr uint32_t FIT = (MAX_SMEM - 1024 - BAR_BYTES) / STAGE;
   static constexpr uint32_t MAX_STAGES = FIT > 8 ? 8 : FIT;
+  // ring of a CTA that shares its SM with a second one (113 KB each)
+  static constexpr uint32_t HALF_STAGES = (113 * 1024 - 1024 - BAR_BYTES) / STAGE;
   static constexpr uint32_t PARTIAL = NT * 128 * 4;  // overlays the ring after the main loop
   static constexpr uint32_t ACC_COLS = NT < 32 ? 32 : NT;
   static constexpr uint32_t SFP_COL = ACC_COLS;
   static constexpr uint32_t SFQ_COL = SFP_COL + 4 * GROUPS;
-  static constexpr uint32_t COLS = SFQ_COL + 4 * GROUPS * QB;
-  static constexpr uint32_t TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static constexpr uint32_t COLS = SFQ_COL + 4 * GROUPS;
+  static constexpr uint32_t TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+  static_assert(NT <= 128 && COLS <= 256, "a tile's rows lie in one scale band, two CTAs share an SM's TMEM");
   static uint32_t smem_bytes(uint32_t stages) {
     const uint32_t ring = stages * STAGE;
     return (ring > PARTIAL ? ring : PARTIAL) + BAR_BYTES + 1024;
@@ -202,7 +247,7 @@ __global__ void __launch_bounds__(256, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + bar_off + 144);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_ptr + bar_off + 148);
 
-  const uint32_t warp = warp_id(), lane = lane_id();
+  const uint32_t warp = __shfl_sync(0xffffffffu, warp_id(), 0), lane = lane_id();
   if (warp == 0 && lane == 0) {
     for (uint32_t s = 0; s < S; ++s) {
       mbar_init(bar_full + 8 * s, 1);
@@ -237,11 +282,9 @@ __global__ void __launch_bounds__(256, 1)
   // this CTA's atoms of K (at least one: splits <= k_atoms)
   const uint32_t k0 = uint32_t(uint64_t(p.k_atoms) * rank / p.splits);
   const uint32_t k1 = uint32_t(uint64_t(p.k_atoms) * (rank + 1) / p.splits);
-  const uint32_t q_bands = (p.nq + 127) / 128 - q0 / 128;  // scale bands left from this tile on
-  const uint32_t qb = q_bands < Cfg::QB ? q_bands : Cfg::QB;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t stage = 0, phase = 0, issued = 0;
       bool ok = true;
       const uint64_t hint_p = policy_evict_first(), hint_q = policy_evict_last();
@@ -254,13 +297,11 @@ __global__ void __launch_bounds__(256, 1)
         const uint32_t g0 = kb * Cfg::GROUPS;
         const uint32_t ng = min(Cfg::GROUPS, p.groups - g0);
         const uint32_t bar = bar_full + 8 * stage;
-        mbar_arrive_expect_tx(bar, Cfg::P_BYTES + Cfg::Q_BYTES + ng * 512u * (1u + qb));
+        mbar_arrive_expect_tx(bar, Cfg::P_BYTES + Cfg::Q_BYTES + ng * 1024u);
         tma_load_2d(sP + stage * Cfg::P_BYTES, &tmP, int32_t(kb * 128u), int32_t(p0), bar, hint_p);
         tma_load_2d(sQ + stage * Cfg::Q_BYTES, &tmQ, int32_t(kb * 128u), int32_t(q0), bar, hint_q);
         bulk_load(sSP + stage * Cfg::SFP_BYTES, p.sf_p + (uint64_t(tp) * p.groups + g0) * 512u, ng * 512u, bar);
-        for (uint32_t b = 0; b < qb; ++b)
-          bulk_load(sSQ + stage * Cfg::SFQ_BYTES + b * Cfg::SFP_BYTES,
-                    p.sf_q + (uint64_t(q0 / 128 + b) * p.groups + g0) * 512u, ng * 512u, bar);
+        bulk_load(sSQ + stage * Cfg::SFQ_BYTES, p.sf_q + (uint64_t(q0 / 128) * p.groups + g0) * 512u, ng * 512u, bar);
         ++issued;
         if (++stage == S) { stage = 0; phase ^= 1u; }
       }
@@ -276,7 +317,7 @@ __global__ void __launch_bounds__(256, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t stage = 0, phase = 0;
       bool ok = true;
       for (uint32_t kb = k0; kb < k1; ++kb) {
@@ -287,25 +328,19 @@ __global__ void __launch_bounds__(256, 1)
         }
         const uint32_t ng = min(Cfg::GROUPS, p.groups - kb * Cfg::GROUPS);
         const uint32_t steps = min(4u, (p.row_bytes - kb * 128u + 31u) / 32u);
-#pragma unroll
-        for (uint32_t g = 0; g < Cfg::GROUPS; ++g) {
-          if (g < ng) {
-            tmem_cp_scales<1>(tmem_base + Cfg::SFP_COL + 4 * g,
-                              sdesc_scale_tile(sSP + stage * Cfg::SFP_BYTES + g * 512u));
-#pragma unroll
-            for (uint32_t b = 0; b < Cfg::QB; ++b)
-              if (b < qb)
-                tmem_cp_scales<1>(tmem_base + Cfg::SFQ_COL + 4 * (Cfg::QB * g + b),
-                                  sdesc_scale_tile(sSQ + stage * Cfg::SFQ_BYTES + b * Cfg::SFP_BYTES + g * 512u));
-          }
-        }
-        const uint32_t a0 = sP + stage * Cfg::P_BYTES, b0 = sQ + stage * Cfg::Q_BYTES;
-#pragma unroll
-        for (uint32_t s = 0; s < 4; ++s) {
-          if (s < steps)
-            umma_mx<1, FMT>(tmem_base, sdesc_k_sw128(a0 + 32u * s), sdesc_k_sw128(b0 + 32u * s),
-                            idesc_mx<FMT>(128, NT, Atom::sf_id(s)), tmem_base + Cfg::SFP_COL + 4 * Atom::group(s),
-                            tmem_base + Cfg::SFQ_COL + 4 * Cfg::QB * Atom::group(s), (kb != k0 || s != 0) ? 1u : 0u);
+        const uint32_t sfp = tmem_base + Cfg::SFP_COL, sfq = tmem_base + Cfg::SFQ_COL;
+        const uint64_t tile_p = sdesc_scale_tile(sSP + stage * Cfg::SFP_BYTES);
+        const uint64_t tile_q = sdesc_scale_tile(sSQ + stage * Cfg::SFQ_BYTES);
+        const uint64_t dp = sdesc_k_sw128(sP + stage * Cfg::P_BYTES), dq = sdesc_k_sw128(sQ + stage * Cfg::Q_BYTES);
+        const uint32_t acc = kb != k0 ? 1u : 0u;
+        if (steps == 4) {
+          using Stage = MxStage<1, FMT, NT, 1, true>;
+          Stage::copy_scales(sfp, sfq, tile_p, tile_q, 0);
+          Stage::mma(tmem_base, dp, dq, sfp, sfq, 4, acc);
+        } else {
+          using Stage = MxStage<1, FMT, NT, 1, false>;
+          Stage::copy_scales(sfp, sfq, tile_p, tile_q, ng);
+          Stage::mma(tmem_base, dp, dq, sfp, sfq, steps, acc);
         }
         umma_commit<1>(bar_empty + 8 * stage);
         if (++stage == S) { stage = 0; phase ^= 1u; }
@@ -383,6 +418,375 @@ __global__ void __launch_bounds__(256, 1)
   }
   // no CTA leaves while another one may still read its partial sums
   if (p.splits > 1) cluster_sync();
+}
+
+// ---------------------------------------------------------------------------------
+// mx_gemm_pair_kernel: 256 x TN tiles of C per CTA pair (cta_group::2), persistent
+// ---------------------------------------------------------------------------------
+// Each CTA of the pair loads its 128 rows of A, half of the tile's rows of B and, since
+// both SMs multiply by every column's scale, its own A scale band and all of B's. The
+// leader issues the scale copies (cta_group::2: each CTA's TMEM from its own shared
+// memory) and the MMAs. TMEM: two accumulator slots of MMA_N columns, then two buffers of
+// scale columns, used by alternate stages. A tile of one MMA width uses the slots in turn
+// (the epilogue of tile t overlaps the main loop of t + 1); TN = 384 uses both.
+struct MxPairParams {
+  uint32_t M, N, row_bytes;
+  uint32_t m_tiles, n_tiles, num_tiles, k_atoms, group_m;
+  const float* ts_a;
+  const float* ts_b;
+  uint8_t* c;
+  uint64_t ldc;   // elements
+  uint32_t vec;   // C rows are 32-byte aligned
+  uint32_t* status;
+  uint64_t wait_ns;
+};
+
+template <int FMT, int TN>
+struct MxPairCfg {
+  static constexpr uint32_t MMA_N = TN == 384 ? 192 : TN;
+  static constexpr uint32_t NH = TN / MMA_N;
+  static constexpr uint32_t GROUPS = MxAtom<FMT>::GROUPS;
+  // 128-row scale bands that a tile's TN columns touch (a 192-wide tile starts at a band
+  // or in the middle of one)
+  static constexpr uint32_t BANDS = TN == 128 ? 1 : TN == 384 ? 3 : 2;
+  static constexpr uint32_t A_BYTES = 128 * 128;
+  static constexpr uint32_t B_HALF = MMA_N / 2 * 128;  // one MMA's B rows of this CTA
+  static constexpr uint32_t B_BYTES = NH * B_HALF;
+  static constexpr uint32_t SFA_BYTES = GROUPS * 512;
+  static constexpr uint32_t SFB_BYTES = BANDS * GROUPS * 512;
+  static constexpr uint32_t STAGE = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+  static constexpr uint32_t BAR_BYTES = 256;
+  static constexpr uint32_t MAX_SMEM = 232448;
+  static constexpr uint32_t EPI_GROUPS = MMA_N / 64;      // 64 columns per epilogue warp
+  static constexpr uint32_t EPI_WARPS = 4 * EPI_GROUPS;
+  static constexpr uint32_t EPI_BYTES = EPI_WARPS * 2048; // staging of C rows at odd pitches
+  static constexpr uint32_t FIT = (MAX_SMEM - 1024 - BAR_BYTES - EPI_BYTES) / STAGE;
+  static constexpr uint32_t STAGES = FIT > 8 ? 8 : FIT;
+  static constexpr uint32_t SMEM = STAGES * STAGE + EPI_BYTES + BAR_BYTES + 1024;
+  static constexpr uint32_t SF_COLS = 4 * GROUPS * (1 + BANDS);
+  static constexpr uint32_t SF_COL = 2 * MMA_N;
+  static constexpr uint32_t THREADS = 128 + 32 * EPI_WARPS;
+  static_assert(SF_COL + 2 * SF_COLS <= 512, "accumulators and scales fit TMEM");
+  static_assert(SMEM > MAX_SMEM / 2, "one CTA per SM: a second one could wait for its TMEM");
+};
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* m, int32_t x, int32_t y, int32_t z,
+                                                 uint32_t cluster_bar, uint64_t hint) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(dst),
+      "l"(m), "r"(x), "r"(y), "r"(z), "r"(cluster_bar), "l"(hint)
+      : "memory");
+}
+
+// 32 consecutive fp32 accumulators of one C row, scaled and rounded, as whole 32-byte
+// sectors (a 32-byte aligned address).
+template <int CD>
+__device__ __forceinline__ void store_c32(uint8_t* c, uint64_t index, const uint32_t (&r)[32], float scale) {
+  using E = typename OutElem<CD>::E;
+  typename E::T* d = reinterpret_cast<typename E::T*>(c) + index;
+  if constexpr (CD == DT_F32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(__uint_as_float(r[8 * j + i]) * scale);
+      st_global_v8(d + 8 * j, w);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        w[i] = E::pack(__uint_as_float(r[16 * j + 2 * i]) * scale, __uint_as_float(r[16 * j + 2 * i + 1]) * scale);
+      st_global_v8(d + 16 * j, w);
+    }
+  }
+}
+
+// The same for a warp's 32 rows x 32 columns at any pitch and column count: 64 bytes of
+// each row go through the warp's shared buffer (16-byte chunk j of row l at chunk
+// j ^ (l / 2 % 4), so neither side has bank conflicts) and leave element by element along
+// the rows. One lane per row storing its own elements touched 32 sectors per store: 777 x
+// 5001 x 2200 took 73 us that way.
+template <int CD>
+__device__ __forceinline__ void store_c32_any(uint8_t* c, uint64_t ldc, uint32_t row0, uint32_t rows, uint32_t col0,
+                                              uint32_t cols, const uint32_t (&r)[32], float scale, uint32_t buf) {
+  using E = typename OutElem<CD>::E;
+  using T = typename E::T;
+  const uint32_t lane = lane_id();
+  constexpr uint32_t W = 64 / sizeof(T);  // columns per pass
+#pragma unroll
+  for (uint32_t x = 0; x < 32; x += W) {
+    uint32_t w[16];
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      if constexpr (CD == DT_F32) w[i] = __float_as_uint(__uint_as_float(r[x + i]) * scale);
+      else w[i] = E::pack(__uint_as_float(r[x + 2 * i]) * scale, __uint_as_float(r[x + 2 * i + 1]) * scale);
+    }
+    __syncwarp();
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+      st_shared_v4(buf + lane * 64u + ((j ^ (lane / 2 & 3u)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    __syncwarp();
+    const uint32_t i = lane % W;
+#pragma unroll 4
+    for (uint32_t l = lane / W; l < rows; l += 32 / W) {
+      if (x + i < cols) {
+        const uint32_t a = buf + l * 64u + (((i * uint32_t(sizeof(T)) / 16) ^ (l / 2 & 3u)) << 4) + i * uint32_t(sizeof(T)) % 16;
+        T v;
+        if constexpr (CD == DT_F32) {
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+        } else {
+          uint16_t u;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(a) : "memory");
+          v = *reinterpret_cast<T*>(&u);
+        }
+        reinterpret_cast<T*>(c)[uint64_t(row0 + l) * ldc + col0 + x + i] = v;
+      }
+    }
+  }
+}
+
+template <int FMT, int CD, int TN>
+__global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
+    mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                        const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+                        const MxPairParams p) {
+  using Cfg = MxPairCfg<FMT, TN>;
+  using Atom = MxAtom<FMT>;
+  constexpr uint32_t S = Cfg::STAGES, NH = Cfg::NH;
+  extern __shared__ uint8_t smem_raw[];
+  // Same offsets in both CTAs: the MMA and the scale copies read the peer's shared memory
+  // at the leader's addresses, commits land on the peer's barriers.
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t sA = base, sB = sA + S * Cfg::A_BYTES;
+  const uint32_t sSA = sB + S * Cfg::B_BYTES, sSB = sSA + S * Cfg::SFA_BYTES;
+  const uint32_t sEpi = base + S * Cfg::STAGE, sBar = sEpi + Cfg::EPI_BYTES;
+  uint8_t* bar_ptr = smem_raw + (sBar - raw);
+  // full[8], empty[8], tfull[2], tempty[2], done, the TMEM address, the abort flag, the two
+  // producers' issued-stage counts
+  const uint32_t bar_full = sBar, bar_empty = sBar + 64, bar_tfull = sBar + 128, bar_tempty = sBar + 144;
+  const uint32_t bar_done = sBar + 160;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_ptr + 168);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(bar_ptr + 172);
+  const uint32_t abort_addr = sBar + 172;
+  volatile uint32_t* issued_words = reinterpret_cast<volatile uint32_t*>(bar_ptr + 176);
+  const uint32_t issued_addr = sBar + 176;
+
+  const uint32_t warp = __shfl_sync(0xffffffffu, warp_id(), 0), lane = lane_id();
+  // the cluster's rank in a form that the compiler knows to be uniform
+  const uint32_t rank = blockIdx.x & 1u, peer = rank ^ 1u;
+  if (warp == 0 && lane == 0) {
+    for (uint32_t s = 0; s < S; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (uint32_t a = 0; a < 2; ++a) {
+      mbar_init(bar_tfull + 8 * a, 1);
+      mbar_init(bar_tempty + 8 * a, Cfg::EPI_WARPS * 2);
+    }
+    mbar_init(bar_done, 1);
+    *abort_flag = 0u;
+    issued_words[0] = 0u;
+    issued_words[1] = 0u;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmSA);
+    tma_prefetch_desc(&tmSB);
+  }
+  if (warp == 1) {
+    tmem_alloc<2>(smem_u32(tmem_slot), 512);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // Raises both CTAs' abort flags (the peer is alive: see the teardown).
+  auto fail = [&](uint32_t code) {
+    *abort_flag = 1u;
+    st_shared_cluster_u32(mapa_shared(abort_addr, peer), 1u);
+    if (p.status) atomicOr(p.status, code | ST_ABORTED);
+  };
+  auto acc_slot = [](uint32_t it, uint32_t h) -> uint32_t { return NH == 1 ? (it & 1u) : h; };
+  auto acc_use = [](uint32_t it) -> uint32_t { return NH == 1 ? (it >> 1) : it; };
+  const uint32_t first_tile = blockIdx.x / 2, tile_stride = gridDim.x / 2;
+
+  if (warp == 0) {
+    // =============================== TMA producer ===============================
+    if (elect_one()) {
+      uint32_t stage = 0, phase = 0, issued = 0;
+      bool ok = true;
+      const uint64_t hint_a = policy_evict_last(), hint_b = policy_evict_first();
+      const uint32_t leader_full0 = mapa_shared(bar_full, 0);
+      for (uint32_t tile = first_tile; tile < p.num_tiles && ok; tile += tile_stride) {
+        uint32_t bm, bn;
+        tile_to_bmn(tile, p.m_tiles, p.n_tiles, p.group_m, bm, bn);
+        const int32_t a_row = int32_t((2 * bm + rank) * 128);
+        const int32_t b_row = int32_t(bn * TN + rank * (Cfg::MMA_N / 2));
+        const int32_t b_band = int32_t(bn * TN / 128);
+        for (uint32_t kb = 0; kb < p.k_atoms; ++kb) {
+          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1u, p.wait_ns, abort_flag)) {
+            fail(ST_PRODUCER_EMPTY);
+            ok = false;
+            break;
+          }
+          // both CTAs' bytes are credited to the leader's barrier, which the leader arms
+          if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * stage, 2 * Cfg::STAGE);
+          const uint32_t lf = leader_full0 + 8 * stage;
+          const int32_t x = int32_t(kb * 128u), g = int32_t(kb * Cfg::GROUPS);
+          tma_load_3d_pair(sSA + stage * Cfg::SFA_BYTES, &tmSA, 0, g, int32_t(2 * bm + rank), lf, hint_a);
+          tma_load_3d_pair(sSB + stage * Cfg::SFB_BYTES, &tmSB, 0, g, b_band, lf, hint_b);
+          tma_load_2d_pair(sA + stage * Cfg::A_BYTES, &tmA, x, a_row, lf, hint_a);
+#pragma unroll
+          for (uint32_t h = 0; h < NH; ++h)
+            tma_load_2d_pair(sB + stage * Cfg::B_BYTES + h * Cfg::B_HALF, &tmB, x, b_row + int32_t(h * Cfg::MMA_N), lf,
+                             hint_b);
+          ++issued;
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (rank == 0) issued_words[0] = issued;
+      else st_shared_cluster_u32(mapa_shared(issued_addr + 4, 0), issued);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ============================ MMA issuer (leader) ============================
+    if (rank != 0) {
+    } else if (elect_one()) {
+      uint32_t stage = 0, phase = 0, it = 0, sf_buf = 0;
+      bool ok = true;
+      for (uint32_t tile = first_tile; tile < p.num_tiles && ok; tile += tile_stride, ++it) {
+        uint32_t bm, bn;
+        tile_to_bmn(tile, p.m_tiles, p.n_tiles, p.group_m, bm, bn);
+        const uint32_t band_shift = bn * TN % 128 / 32;  // scale columns before the tile's first
+        for (uint32_t kb = 0; kb < p.k_atoms; ++kb) {
+          if (!mbar_wait(bar_full + 8 * stage, phase, p.wait_ns, abort_flag)) {
+            fail(ST_MMA_FULL);
+            ok = false;
+            break;
+          }
+          const uint32_t sfa = tmem_base + Cfg::SF_COL + sf_buf * Cfg::SF_COLS, sfb = sfa + 4 * Cfg::GROUPS;
+          sf_buf ^= 1u;
+          const uint64_t tile_a = sdesc_scale_tile(sSA + stage * Cfg::SFA_BYTES);
+          const uint64_t tile_b = sdesc_scale_tile(sSB + stage * Cfg::SFB_BYTES);
+          const uint64_t da = sdesc_k_sw128(sA + stage * Cfg::A_BYTES), db = sdesc_k_sw128(sB + stage * Cfg::B_BYTES);
+          const uint32_t steps = min(4u, (p.row_bytes - kb * 128u + 31u) / 32u);
+          const uint32_t acc = kb ? 1u : 0u;
+          // boxes past the last scale tile read as zero, so every copy has its source
+          MxStage<2, FMT, Cfg::MMA_N, Cfg::BANDS, true>::copy_scales(sfa, sfb, tile_a, tile_b, 0);
+#pragma unroll
+          for (uint32_t h = 0; h < NH; ++h) {
+            const uint32_t slot = acc_slot(it, h);
+            if (kb == 0) {
+              if (!mbar_wait(bar_tempty + 8 * slot, (acc_use(it) & 1u) ^ 1u, p.wait_ns, abort_flag)) {
+                fail(ST_MMA_TMEM_EMPTY);
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+            }
+            const uint32_t sfb_h = sfb + (NH == 1 ? band_shift : h * Cfg::MMA_N / 32);
+            const uint32_t d = tmem_base + slot * Cfg::MMA_N;
+            const uint64_t db_h = db + h * (Cfg::B_HALF >> 4);
+            if (steps == 4) MxStage<2, FMT, Cfg::MMA_N, Cfg::BANDS, true>::mma(d, da, db_h, sfa, sfb_h, 4, acc);
+            else MxStage<2, FMT, Cfg::MMA_N, Cfg::BANDS, false>::mma(d, da, db_h, sfa, sfb_h, steps, acc);
+            if (kb + 1 == p.k_atoms) umma_commit_pair(bar_tfull + 8 * slot, uint16_t(3u));
+          }
+          if (!ok) break;
+          umma_commit_pair(bar_empty + 8 * stage, uint16_t(3u));
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
+      }
+      umma_commit<2>(bar_done);
+      if (!mbar_wait_bounded(bar_done, 0, p.wait_ns)) fail(ST_DRAIN);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ================================ epilogue ================================
+    // Warp 4 + 4e + q drains lanes 32q ... 32q + 31, columns 64e ... 64e + 63 of each slot
+    // and hands the slot back before it converts and stores. A lane owns one C row: its 64
+    // columns are whole 32-byte sectors, stored straight from registers.
+    const uint32_t q = warp & 3u, e = (warp - 4) >> 2;
+    float scale = 1.0f;
+    if (p.ts_a) scale *= __ldg(p.ts_a);
+    if (p.ts_b) scale *= __ldg(p.ts_b);
+    const uint32_t leader_tempty0 = mapa_shared(bar_tempty, 0);
+    uint32_t it = 0;
+    bool ok = true;
+    for (uint32_t tile = first_tile; tile < p.num_tiles && ok; tile += tile_stride, ++it) {
+      uint32_t bm, bn;
+      tile_to_bmn(tile, p.m_tiles, p.n_tiles, p.group_m, bm, bn);
+      const uint32_t row0 = (2 * bm + rank) * 128 + 32 * q;
+#pragma unroll 1
+      for (uint32_t h = 0; h < NH; ++h) {
+        const uint32_t slot = acc_slot(it, h);
+        uint32_t okw = 0;
+        if (lane == 0) okw = mbar_wait(bar_tfull + 8 * slot, acc_use(it) & 1u, p.wait_ns, abort_flag) ? 1u : 0u;
+        okw = __shfl_sync(0xffffffffu, okw, 0);
+        if (!okw) {
+          if (lane == 0) fail(ST_EPI_TMEM_FULL);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t t0 = tmem_base + ((32u * q) << 16) + slot * Cfg::MMA_N + 64u * e;
+        uint32_t r[2][32];
+        tmem_ld_x32(t0, r[0]);
+        tmem_ld_x32(t0 + 32, r[1]);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty0 + 8 * slot);
+        const uint32_t col = bn * TN + h * Cfg::MMA_N + 64u * e;
+        if (row0 < p.M) {
+#pragma unroll
+          for (uint32_t x = 0; x < 2; ++x) {
+            const uint32_t cx = col + 32u * x;
+            if (p.vec && cx + 32 <= p.N) {
+              if (row0 + lane < p.M) store_c32<CD>(p.c, uint64_t(row0 + lane) * p.ldc + cx, r[x], scale);
+            } else if (cx < p.N) {
+              store_c32_any<CD>(p.c, p.ldc, row0, min(32u, p.M - row0), cx, p.N - cx, r[x], scale,
+                                sEpi + (warp - 4) * 2048u);
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  // ---- teardown: as the plain pair kernel's (gemm_sm100.cuh): after an abort the leader
+  // waits for every stage still in flight before either CTA leaves ----
+  tc_fence_before();
+  cluster_sync();
+  if (*abort_flag) {
+    if (warp == 0 && lane == 0 && rank == 0) {
+      const uint32_t il = issued_words[0], ip = issued_words[1];
+      const uint32_t hi = il > ip ? il : ip;
+      for (uint32_t i = hi > S ? hi - S : 0u; i < hi; ++i) {
+        const uint32_t bar = bar_full + 8 * (i % S);
+        if (i >= il) mbar_arrive_expect_tx(bar, Cfg::STAGE);
+        else if (i >= ip) mbar_complete_tx(bar, Cfg::STAGE);
+        if (!mbar_wait_bounded(bar, (i / S) & 1u, p.wait_ns)) {
+          fail(ST_DRAIN);
+          break;
+        }
+      }
+    }
+    cluster_sync();
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<2>(tmem_base, 512);
+  }
 }
 
 }  // namespace b200
