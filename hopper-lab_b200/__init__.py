@@ -64,6 +64,8 @@ EXPORTS = [
 GATHER_MULTICAST, GATHER_PEERS = 1, 2
 MX_FORMATS = {"mxfp8": 0, "mxfp4": 1, "nvfp4": 2}
 MX_NORM_MAX_COLS = 32768
+MX_SCALE_BYTES = 272
+_MX_GAP = 512  # MX_SCALE_BYTES in whole 256-byte units
 
 
 class GemmArgs(C.Structure):
@@ -393,7 +395,6 @@ def quantize_e4m3(x, q=None, scale=None, stream=None):
 # ------------------------------------------------------------------ microscaled operands
 # These calls are short kernels, so their host side is kept short too: one allocation for a
 # microscaled matrix, views of it only when asked for, raw stream handles.
-_MX_BLOCK = {"mxfp8": 32, "mxfp4": 32, "nvfp4": 16}
 
 
 def mx_layout(fmt: str, rows: int, cols: int) -> tuple[int, int]:
@@ -448,27 +449,31 @@ class MxTensor:
 
     @classmethod
     def _new(cls, rows, cols, fmt, device):
-        # one buffer: scale tiles, 256 bytes with a tensor scale and its scratch, element rows
-        blk = _MX_BLOCK[fmt]
+        # one buffer: scale tiles, the tensor scale and its scratch, element rows
         kp = (cols + 31) // 32 * 32
-        scale_bytes = (rows + 127) // 128 * ((kp // blk + 3) // 4) * 512
-        row_bytes = kp if fmt == "mxfp8" else kp // 2
-        self = object.__new__(cls)
+        if fmt == "nvfp4":
+            groups, row_bytes, code = (kp + 63) // 64, kp // 2, 2
+        elif fmt == "mxfp8":
+            groups, row_bytes, code = (kp + 127) // 128, kp, 0
+        else:
+            groups, row_bytes, code = (kp + 127) // 128, kp // 2, 1
+        scale_bytes = (rows + 127) // 128 * groups * 512
         torch = _torch()
-        self._own = buf = torch.empty(scale_bytes + 256 + rows * row_bytes, dtype=torch.uint8, device=device)
+        self = object.__new__(cls)
+        self._own = buf = torch.empty(scale_bytes + _MX_GAP + rows * row_bytes, dtype=torch.uint8, device=device)
         self._off = scale_bytes
         ptr = buf.data_ptr()
         self._data = self._scales = self._ts = None
         self.fmt, self.rows, self.cols, self.device = fmt, rows, cols, buf.device
-        self._desc = MxDesc(MX_FORMATS[fmt], 0, rows, cols, row_bytes, ptr + scale_bytes + 256, ptr, None)
-        self._ref = C.byref(self._desc)
+        self._desc = desc = MxDesc(code, 0, rows, cols, row_bytes, ptr + scale_bytes + _MX_GAP, ptr, None)
+        self._ref = C.byref(desc)
         return self
 
     @property
     def data(self):
         if self._data is None:
             ld = self._desc.ld
-            self._data = self._own.as_strided((self.rows, ld), (ld, 1), self._off + 256)
+            self._data = self._own.as_strided((self.rows, ld), (ld, 1), self._off + _MX_GAP)
         return self._data
 
     @property
@@ -497,9 +502,9 @@ class MxTensor:
         self._desc.tensor_scale = None if ts is None else ts.data_ptr()
 
     def _scratch(self):
-        """16 bytes for a tensor scale to be found into."""
+        """Room for a tensor scale to be found into."""
         if self._own is None:  # data and scales are the caller's: a buffer beside them
-            self._own = _torch().empty(256, dtype=_torch().uint8, device=self.device)
+            self._own = _torch().empty(_MX_GAP, dtype=_torch().uint8, device=self.device)
         self._ts = None
         self._desc.tensor_scale = self._own.data_ptr() + self._off
 
@@ -508,15 +513,24 @@ class MxTensor:
         return self.rows, self.cols
 
 
-_MX_IN = {}
+_MX_TORCH = {}  # torch dtype -> code and the names of output types -> (torch dtype, code)
+
+
+def _mx_types():
+    if not _MX_TORCH:
+        torch = _torch()
+        for dt, code, names in ((torch.float16, DT_F16, ("f16", "fp16", "float16")),
+                                (torch.bfloat16, DT_BF16, ("bf16", "bfloat16")),
+                                (torch.float32, DT_F32, ("f32", "fp32", "float32"))):
+            _MX_TORCH[dt] = code
+            for name in names + (code,):
+                _MX_TORCH[name] = (dt, code)
+    return _MX_TORCH
 
 
 def _mx_input(name, t):
     """dtype code and row stride of a 2-D fp tensor with unit column stride."""
-    if not _MX_IN:
-        torch = _torch()
-        _MX_IN.update({torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.float32: DT_F32})
-    dt = _MX_IN.get(t.dtype)
+    dt = (_MX_TORCH or _mx_types()).get(t.dtype)
     if dt is None:
         raise TypeError(f"{name} must be float16, bfloat16 or float32, not {t.dtype}")
     shape = t.shape
@@ -528,20 +542,19 @@ def _mx_input(name, t):
     return dt, ld if shape[0] > 1 else max(shape[1], 1)
 
 
-_MX_OUT = {}
-
-
-def _mx_out_dtype(name):
-    dt = _MX_OUT.get(name)
-    if dt is None:
-        dt = _MX_OUT[name] = _torch_dtype(_dtype_code(name))
-    return dt
+def _mx_output(name, rows, cols, device):
+    """A new matrix of the named output type, its code and row stride."""
+    kind = (_MX_TORCH or _mx_types()).get(name)
+    if type(kind) is not tuple:
+        raise ValueError(f"output type {name!r} is not f16, bf16 or f32")
+    ld = max(cols, 1)
+    return _torch().empty_strided((rows, cols), (ld, 1), dtype=kind[0], device=device), kind[1], ld
 
 
 def _mx_out(out, rows, cols, fmt, device, tensor_scale):
-    if fmt not in MX_FORMATS:
-        raise ValueError(f"unknown format {fmt!r}")
     if out is None:
+        if fmt not in MX_FORMATS:
+            raise ValueError(f"unknown format {fmt!r}")
         out = MxTensor._new(rows, cols, fmt, device)
         if tensor_scale is not None:
             out.tensor_scale = tensor_scale
@@ -553,24 +566,25 @@ def _mx_out(out, rows, cols, fmt, device, tensor_scale):
 
 
 class _On:
-    """Current device and stream of one call: what the call allocates belongs to the stream
-    that its kernels run on. ``stream``: a torch stream or a raw handle."""
+    """Makes a call's device and stream the current ones, so that what it allocates belongs to
+    the stream that its kernels run on. ``stream``: None (the device's current one), a torch
+    stream or a raw handle."""
 
-    __slots__ = ("_device", "_stream", "handle")
+    __slots__ = ("_device", "_stream")
 
     def __init__(self, device, stream):
-        torch = _torch()
-        self._device = torch.cuda.device(device)
-        self._stream = torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
+        cuda = _torch().cuda
+        if device.type != "cuda":
+            raise ValueError(f"tensors must be on a CUDA device, not {device}")
+        self._device = cuda.device(device)
+        if stream is not None:
+            stream = cuda.stream(cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
+        self._stream = stream
 
     def __enter__(self):
-        torch = _torch()
         self._device.__enter__()
-        self.handle = (self._stream or torch.cuda.current_stream()).cuda_stream
         if self._stream is not None:
-            self._stream = torch.cuda.stream(self._stream)
             self._stream.__enter__()
-        return self
 
     def __exit__(self, *exc):
         if self._stream is not None:
@@ -578,27 +592,14 @@ class _On:
         self._device.__exit__(*exc)
 
 
-class _Here:
-    """_On for the usual call: the current device and its current stream."""
-
-    __slots__ = ("handle",)
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        pass
-
-
-def _on(device, stream):
-    if device.type != "cuda":
-        raise ValueError(f"tensors must be on a CUDA device, not {device}")
-    cuda = _torch().cuda
-    if stream is None and cuda.current_device() == device.index:
-        here = _Here()
-        here.handle = _torch()._C._cuda_getCurrentRawStream(device.index)
-        return here
-    return _On(device, stream)
+def _here(device, stream):
+    """Handle of the current stream for a call on the current device and stream, else None:
+    the call then makes them current (_On) and starts over."""
+    if stream is None and device.index is not None:
+        cuda = _torch()._C
+        if cuda._cuda_getDevice() == device.index:
+            return cuda._cuda_getCurrentRawStream(device.index)
+    return None
 
 
 def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=None, out: MxTensor | None = None,
@@ -608,16 +609,19 @@ def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=
     positive fp32 on the device, used as given; None finds max|x| / 2688 in an extra pass.
     ``out`` is written in place and takes the tensor scale."""
     dt, ldx = _mx_input("x", x)
+    device = x.device
+    here = _here(device, stream)
+    if here is None:
+        with _On(device, stream):
+            return quantize_mx(x, fmt, transpose=transpose, tensor_scale=tensor_scale, out=out)
     rows, cols = x.shape
     if transpose:
         rows, cols = cols, rows
-    device = x.device
-    with _on(device, stream) as on:
-        t = _mx_out(out, rows, cols, fmt, device, tensor_scale)
-        find = fmt == "nvfp4" and tensor_scale is None
-        if find:
-            t._scratch()
-        rc = (_LIB or lib()).b200_mx_quantize(x.data_ptr(), dt, ldx, transpose, find, t._ref, on.handle)
+    t = _mx_out(out, rows, cols, fmt, device, tensor_scale)
+    find = fmt == "nvfp4" and tensor_scale is None
+    if find:
+        t._scratch()
+    rc = (_LIB or lib()).b200_mx_quantize(x.data_ptr(), dt, ldx, transpose, find, t._ref, here)
     if rc != OK:
         raise B200Error(rc, "b200_mx_quantize")
     return t
@@ -626,13 +630,17 @@ def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=
 def dequantize_mx(t: MxTensor, out=None, *, out_dtype="bf16", stream=None):
     """The values a microscaled matrix stands for, rounded once to f16, bf16 or f32."""
     device = t.device
-    with _on(device, stream) as on:
-        if out is None:
-            out = _torch().empty((t.rows, t.cols), dtype=_mx_out_dtype(out_dtype), device=device)
-        elif tuple(out.shape) != t.shape or out.device != device:
+    here = _here(device, stream)
+    if here is None:
+        with _On(device, stream):
+            return dequantize_mx(t, out, out_dtype=out_dtype)
+    if out is None:
+        out, dt, ldy = _mx_output(out_dtype, t.rows, t.cols, device)
+    else:
+        if tuple(out.shape) != t.shape or out.device != device:
             raise ValueError(f"out is {tuple(out.shape)} on {out.device}, needed {t.shape} on {device}")
         dt, ldy = _mx_input("out", out)
-        rc = (_LIB or lib()).b200_mx_dequantize(t._ref, out.data_ptr(), dt, ldy, on.handle)
+    rc = (_LIB or lib()).b200_mx_dequantize(t._ref, out.data_ptr(), dt, ldy, here)
     if rc != OK:
         raise B200Error(rc, "b200_mx_dequantize")
     return out
@@ -646,13 +654,17 @@ def gemm_mx(a: MxTensor, b: MxTensor, c=None, *, out_dtype="bf16", stream=None):
         raise TypeError(f"A and B must have the same format, not {a.fmt} and {b.fmt}")
     if a.cols != b.cols or device != b.device:
         raise ValueError(f"shape or device mismatch: A {a.shape} on {device}, B {b.shape} on {b.device}")
-    with _on(device, stream) as on:
-        if c is None:
-            c = _torch().empty((a.rows, b.rows), dtype=_mx_out_dtype(out_dtype), device=device)
-        elif tuple(c.shape) != (a.rows, b.rows) or c.device != device:
+    here = _here(device, stream)
+    if here is None:
+        with _On(device, stream):
+            return gemm_mx(a, b, c, out_dtype=out_dtype)
+    if c is None:
+        c, dt, ldc = _mx_output(out_dtype, a.rows, b.rows, device)
+    else:
+        if tuple(c.shape) != (a.rows, b.rows) or c.device != device:
             raise ValueError(f"C is {tuple(c.shape)} on {c.device}, needed {(a.rows, b.rows)} on {device}")
         dt, ldc = _mx_input("C", c)
-        rc = (_LIB or lib()).b200_mx_gemm(a._ref, b._ref, c.data_ptr(), dt, ldc, on.handle)
+    rc = (_LIB or lib()).b200_mx_gemm(a._ref, b._ref, c.data_ptr(), dt, ldc, here)
     if rc != OK:
         raise B200Error(rc, "b200_mx_gemm")
     return c
@@ -666,33 +678,39 @@ def rms_norm_mx(x, weight, residual=None, *, eps: float = 1e-6, fmt: str = "mxfp
     ``weight`` has x's type or is float32; ``tensor_scale`` ("nvfp4") is used as given, None
     stands for 1, which suits normalised rows (block maxima from 0.006 to 2688)."""
     dt, ldx = _mx_input("x", x)
-    rows, cols = shape = x.shape
     device = x.device
-    wt = _MX_IN.get(weight.dtype)
+    shape = x.shape
+    rows, cols = shape
+    wt = _MX_TORCH.get(weight.dtype)
     if weight.shape != (cols,) or not weight.is_contiguous() or weight.device != device:
         raise ValueError(f"weight must hold {cols} contiguous elements on {device}")
     if wt != dt and wt != DT_F32:
         raise TypeError(f"weight must be {x.dtype} or float32, not {weight.dtype}")
     if residual is None and residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    with _on(device, stream) as on:
-        if residual is None:
-            args = MxNormArgs(dt, wt, x.data_ptr(), weight.data_ptr(), None, None, ldx, 0, 0, eps, 0)
+    here = _here(device, stream)
+    if here is None:
+        with _On(device, stream):
+            return rms_norm_mx(x, weight, residual, eps=eps, fmt=fmt, tensor_scale=tensor_scale, out=out,
+                               residual_out=residual_out)
+    if residual is None:
+        args = MxNormArgs(dt, wt, x.data_ptr(), weight.data_ptr(), None, None, ldx, 0, 0, eps, 0)
+    else:
+        if residual.shape != shape or residual.device != device:
+            raise ValueError(f"residual must match x: {tuple(shape)} on {device}")
+        rt, ldr = _mx_input("residual", residual)
+        if residual_out is None:
+            residual_out, ht, ldh = _mx_output(dt, rows, cols, device)
         else:
-            if residual_out is None:
-                residual_out = _torch().empty((rows, cols), dtype=x.dtype, device=device)
-            elif residual_out.shape != shape or residual_out.device != device:
+            if residual_out.shape != shape or residual_out.device != device:
                 raise ValueError(f"residual_out must match x: {tuple(shape)} on {device}")
-            if residual.shape != shape or residual.device != device:
-                raise ValueError(f"residual must match x: {tuple(shape)} on {device}")
-            rt, ldr = _mx_input("residual", residual)
             ht, ldh = _mx_input("residual_out", residual_out)
-            if rt != dt or ht != dt:
-                raise TypeError(f"residual and residual_out must be {x.dtype}")
-            args = MxNormArgs(dt, wt, x.data_ptr(), weight.data_ptr(), residual.data_ptr(), residual_out.data_ptr(),
-                              ldx, ldr, ldh, eps, 0)
-        t = _mx_out(out, rows, cols, fmt, device, tensor_scale)
-        rc = (_LIB or lib()).b200_mx_rms_norm(C.byref(args), t._ref, on.handle)
+        if rt != dt or ht != dt:
+            raise TypeError(f"residual and residual_out must be {x.dtype}")
+        args = MxNormArgs(dt, wt, x.data_ptr(), weight.data_ptr(), residual.data_ptr(), residual_out.data_ptr(),
+                          ldx, ldr, ldh, eps, 0)
+    t = _mx_out(out, rows, cols, fmt, device, tensor_scale)
+    rc = (_LIB or lib()).b200_mx_rms_norm(C.byref(args), t._ref, here)
     if rc != OK:
         raise B200Error(rc, "b200_mx_rms_norm")
     return t, residual_out

@@ -78,9 +78,24 @@ struct Elem<3> {
   static __device__ __forceinline__ T store(float v) { return v; }
 };
 
+// Untiled bulk copy into this CTA's shared memory; both addresses and the size are
+// multiples of 16 bytes.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 // 32 bytes in one access (sm_100's widest), for a 32-byte aligned address.
 __device__ __forceinline__ void ld_global_v8(const void* p, uint32_t (&r)[8]) {
   asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p)
+               : "memory");
+}
+// The same, kept in L1: for data that a CTA reads again.
+__device__ __forceinline__ void ld_global_v8_l1(const void* p, uint32_t (&r)[8]) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "l"(p)
                : "memory");
@@ -91,15 +106,43 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&r)[8]) {
                : "memory");
 }
 
-// 16 consecutive elements as fp32. `wide`: the address is 32-byte aligned and all 16
-// exist; otherwise the `n` existing ones are read one by one and the rest are zero.
+// 16 consecutive elements as they lie in memory (two to a register for 16-bit types).
 template <int DT>
-__device__ __forceinline__ void load16(const typename Elem<DT>::T* p, bool wide, int n, float (&v)[16]) {
+struct Raw16 {
   using E = Elem<DT>;
-  if (wide) {
-    if constexpr (sizeof(typename E::T) == 2) {
-      uint32_t r[8];
-      ld_global_v8(p, r);
+  using T = typename E::T;
+  static constexpr bool PACKED = sizeof(T) == 2;
+  uint32_t r[PACKED ? 8 : 16];
+
+  // `wide`: the address is 32-byte aligned and all 16 exist; otherwise the `n` existing
+  // ones are read one by one and the rest are zero.
+  template <bool KEEP = false>
+  __device__ __forceinline__ void load(const T* p, bool wide, int n) {
+    if (wide) {
+      uint32_t(&lo)[8] = *reinterpret_cast<uint32_t(*)[8]>(r);
+      if constexpr (KEEP) ld_global_v8_l1(p, lo);
+      else ld_global_v8(p, lo);
+      if constexpr (!PACKED) {
+        uint32_t(&hi)[8] = *reinterpret_cast<uint32_t(*)[8]>(r + 8);
+        if constexpr (KEEP) ld_global_v8_l1(p + 8, hi);
+        else ld_global_v8(p + 8, hi);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        uint32_t e = 0;
+        if (i < n) {
+          if constexpr (PACKED) e = *reinterpret_cast<const uint16_t*>(p + i);
+          else e = __float_as_uint(p[i]);
+        }
+        if constexpr (!PACKED) r[i] = e;
+        else if (i & 1) r[i / 2] |= e << 16;
+        else r[i / 2] = e;
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&v)[16]) const {
+    if constexpr (PACKED) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float2 f = E::unpack(r[i]);
@@ -107,19 +150,18 @@ __device__ __forceinline__ void load16(const typename Elem<DT>::T* p, bool wide,
         v[2 * i + 1] = f.y;
       }
     } else {
-      uint32_t r[8], s[8];
-      ld_global_v8(p, r);
-      ld_global_v8(p + 8, s);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = __uint_as_float(r[i]);
-        v[8 + i] = __uint_as_float(s[i]);
-      }
+      for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = i < n ? E::load(p[i]) : 0.0f;
   }
+};
+
+// 16 consecutive elements as fp32; `wide` and `n` as above, KEEP: through L1.
+template <int DT, bool KEEP = false>
+__device__ __forceinline__ void load16(const typename Elem<DT>::T* p, bool wide, int n, float (&v)[16]) {
+  Raw16<DT> w;
+  w.template load<KEEP>(p, wide, n);
+  w.unpack(v);
 }
 
 // Store 16 fp32 values rounded to the element type; `wide` and `n` as above.
@@ -144,6 +186,68 @@ __device__ __forceinline__ void store16(typename Elem<DT>::T* p, bool wide, int 
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if (i < n) p[i] = E::store(v[i]);
+  }
+}
+
+// Rows that do not start on 32 bytes: a warp's 512 consecutive elements go element by
+// element, lanes side by side, and change hands in shared memory (256 at a time), so that
+// every lane still owns 16 consecutive ones. A lane loading or storing its own 16 one by
+// one touches 32 sectors per access instead of 2 or 4 (1001 x 5003 to bf16: 34 us that
+// way for the dequantiser). All lanes take part; `p` is the warp's first element, of which
+// `n` exist (n may be negative).
+constexpr int kStageFloats = 272;  // per warp: 256 and one of padding per 16
+template <int DT>
+__device__ __forceinline__ void warp_load16(const typename Elem<DT>::T* p, int64_t n, float* stage, float (&v)[16]) {
+  const uint32_t lane = lane_id();
+#pragma unroll
+  for (uint32_t half = 0; half < 2; ++half) {
+    float t[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t k = 256 * half + 32 * i + lane;
+      t[i] = int64_t(k) < n ? Elem<DT>::load(p[k]) : 0.0f;
+    }
+    __syncwarp();
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t k = 32 * i + lane;
+      stage[k + k / 16] = t[i];
+    }
+    __syncwarp();
+    if (lane / 16 == half) {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) v[i] = stage[lane % 16 * 17 + i];
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ void warp_load16(const typename Elem<DT>::T* p, int64_t n, float* stage, Raw16<DT>& w) {
+  float v[16];
+  warp_load16<DT>(p, n, stage, v);
+  if constexpr (Raw16<DT>::PACKED) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.r[i] = Elem<DT>::pack(v[2 * i], v[2 * i + 1]);  // exact: they came from 16 bits
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w.r[i] = __float_as_uint(v[i]);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void warp_store16(typename Elem<DT>::T* p, int64_t n, float* stage, const float (&v)[16]) {
+  const uint32_t lane = lane_id();
+#pragma unroll
+  for (uint32_t half = 0; half < 2; ++half) {
+    __syncwarp();
+    if (lane / 16 == half) {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) stage[lane % 16 * 17 + i] = v[i];
+    }
+    __syncwarp();
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const uint32_t k = 32 * i + lane;
+      if (int64_t(256 * half + k) < n) p[256 * half + k] = Elem<DT>::store(stage[k + k / 16]);
+    }
   }
 }
 
@@ -176,10 +280,40 @@ __device__ __forceinline__ float e4m3_to_f32(uint32_t byte) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h2)).x;
 }
 
-// Largest magnitude of a block with "holds a NaN or an infinity" folded in: on the bit
-// patterns without the sign, finite values order as integers below 0x7F800000 and every
-// non-finite value is at or above it.
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+// Largest magnitude of n values (n even) as a bit pattern, with "holds a NaN or an
+// infinity" folded in: a NaN survives max.NaN, non-negative patterns order as integers, and
+// every non-finite one is at or above 0x7F800000.
+template <int N>
+__device__ __forceinline__ uint32_t amax_bits(const float* v) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(v[i]), "f"(v[i + 1]));
+  return __float_as_uint(m) & 0x7FFFFFFFu;
+}
+
+// The same of packed 16-bit values, two patterns at a time (their order is that of unsigned
+// integers too): the maximum of the low halves and of the high ones.
+template <int N>
+__device__ __forceinline__ uint32_t amax_packed(const uint32_t* r) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) m = __vimax3_u16x2(m, r[i] & 0x7FFF7FFFu, r[i + 1] & 0x7FFF7FFFu);
+  return m;
+}
+// fp32 pattern of a 16-bit magnitude pattern in the low half; non-finite stays non-finite.
+template <int DT>
+__device__ __forceinline__ uint32_t widen_bits(uint32_t h) {
+  return __float_as_uint(Elem<DT>::unpack(h & 0xFFFFu).x);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t amax_raw(const Raw16<DT>& w) {
+  if constexpr (Raw16<DT>::PACKED) {
+    const uint32_t m = amax_packed<8>(w.r);
+    return widen_bits<DT>(max(m & 0xFFFFu, m >> 16));
+  } else {
+    return amax_bits<16>(reinterpret_cast<const float*>(w.r));
+  }
+}
 
 // Scale byte of an MX block with largest magnitude `amax` (bits as above): the smallest
 // e >= -127 with amax <= QMAX * 2^e, so no element saturates (a floor of the exponent
@@ -219,9 +353,8 @@ __device__ __forceinline__ uint32_t nv_scale_byte(uint32_t amax) {
 // multiply-adds (Markstein, "Computation of elementary functions on the IBM RISC
 // System/6000 processor", 1990) gives the correctly rounded quotient for the 4-bit
 // significand of s, so ties between e2m1 values fall as the definition says. By the same
-// spacing argument as above no other quotient rounds onto a tie. Out-of-range quotients
-// only need to stay above 6 (the residual of an infinite product would be NaN, so
-// huge u keeps the first product).
+// spacing argument as above no other quotient rounds onto a tie. Nothing overflows: u / s
+// is below 10 unless s = 448, the largest scale, and then it is below u.
 struct NvInverse {
   float s, r;
   __device__ __forceinline__ explicit NvInverse(uint32_t byte) {
@@ -230,18 +363,27 @@ struct NvInverse {
   }
   __device__ __forceinline__ float quotient(float u) const {
     const float y = u * r;
-    const float q = fmaf(fmaf(-y, s, u), r, y);
-    return fabsf(y) < 16.0f ? q : y;
+    return fmaf(fmaf(-y, s, u), r, y);
   }
 };
 
-// Quantise 16 consecutive fp32 values of one row and return their bytes and scale byte.
-// Blocks of 32 are shared by lanes 2i and 2i + 1 (all lanes of the warp take part).
+// 16 scaled values to their element bytes.
 template <int FMT>
-__device__ __forceinline__ uint32_t mx_quantize16(float (&v)[16], uint32_t (&out)[4]) {
-  uint32_t amax = 0;
+__device__ __forceinline__ void mx_pack16(const float (&v)[16], uint32_t (&out)[4]) {
+  if constexpr (FMT == MX_FP8) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) amax = max(amax, abs_bits(v[i]));
+    for (int i = 0; i < 4; ++i) out[i] = cvt_e4m3x4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  } else {
+    out[0] = cvt_e2m1x8(v);
+    out[1] = cvt_e2m1x8(v + 8);
+  }
+}
+
+// Quantise 16 consecutive fp32 values of one row, `amax` their largest magnitude's bits, and
+// return their bytes and scale byte. Blocks of 32 are shared by lanes 2i and 2i + 1 (all
+// lanes of the warp take part).
+template <int FMT>
+__device__ __forceinline__ uint32_t mx_quantize16(float (&v)[16], uint32_t amax, uint32_t (&out)[4]) {
   if constexpr (MxFmt<FMT>::BLOCK == 32) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   uint32_t byte;
   if constexpr (FMT == NV_FP4) {
@@ -255,13 +397,7 @@ __device__ __forceinline__ uint32_t mx_quantize16(float (&v)[16], uint32_t (&out
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] *= m;
   }
-  if constexpr (FMT == MX_FP8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = cvt_e4m3x4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  } else {
-    out[0] = cvt_e2m1x8(v);
-    out[1] = cvt_e2m1x8(v + 8);
-  }
+  mx_pack16<FMT>(v, out);
   return byte;
 }
 

@@ -19,14 +19,6 @@ namespace b200 {
 // ---------------------------------------------------------------------------------
 // PTX
 // ---------------------------------------------------------------------------------
-// Untiled bulk copy into this CTA's shared memory; both addresses and the size are
-// multiples of 16 bytes.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
 // Shared-memory descriptor of one 512-byte scale tile: no swizzle, 32 rows of 16 bytes
 // as four 8-row core matrices 128 bytes apart.
 __device__ __forceinline__ uint64_t sdesc_scale_tile(uint32_t saddr) {
@@ -388,8 +380,8 @@ __global__ void __launch_bounds__(256, 1)
   if (p.splits > 1) cluster_sync();
   if (!*abort_flag) {
     float scale = 1.0f;
-    if (p.ts_p) scale *= __ldg(p.ts_p);
-    if (p.ts_q) scale *= __ldg(p.ts_q);
+    if (p.ts_p) scale *= *p.ts_p;
+    if (p.ts_q) scale *= *p.ts_q;
     const uint32_t rows = min(uint32_t(NT), p.nq - q0);
     const uint32_t col = p0 + 4 * lane;
     const uint32_t ncol = col < p.np ? min(4u, p.np - col) : 0u;
@@ -716,8 +708,8 @@ __global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
     // columns are whole 32-byte sectors, stored straight from registers.
     const uint32_t q = warp & 3u, e = (warp - 4) >> 2;
     float scale = 1.0f;
-    if (p.ts_a) scale *= __ldg(p.ts_a);
-    if (p.ts_b) scale *= __ldg(p.ts_b);
+    if (p.ts_a) scale *= *p.ts_a;
+    if (p.ts_b) scale *= *p.ts_b;
     const uint32_t leader_tempty0 = mapa_shared(bar_tempty, 0);
     uint32_t it = 0;
     bool ok = true;

@@ -10,6 +10,7 @@
 // of 32 (a shuffle joins the halves), 16 or 8 bytes out.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "b200gemm.h"
@@ -23,47 +24,108 @@ using namespace b200;
 // ---------------------------------------------------------------------------------
 // per-tensor scale of NV_FP4: amax / (6 * 448)
 // ---------------------------------------------------------------------------------
-// ts[0] the scale, ts[1] the running maximum's bits, ts[2] the count of finished blocks;
-// ts[1] and ts[2] start at zero. The maximum of the finite magnitudes does not depend on
-// the order of the atomics; the last block turns it into the scale.
-template <int DT>
-__global__ void __launch_bounds__(256) mx_amax_kernel(const typename Elem<DT>::T* __restrict__ x, int64_t rows,
-                                                      int64_t cols, int64_t ld, int wide, uint32_t* ts) {
+// The first kernel leaves one maximum of finite magnitudes per cluster of CTAs behind the
+// scale, at most kPartials; every warp of the quantiser reduces them again (the maximum does
+// not depend on the order) and the first CTA writes the scale. No counter or flag has to
+// start at zero, so there is no memset, and the quantiser's launch overlaps the first
+// kernel's end.
+constexpr int kPartials = 64;
+constexpr int kAmaxCluster = 8;
+static_assert(16 + kPartials * 4 <= B200_MX_SCALE_BYTES, "scratch behind the tensor scale");
+
+__global__ void mx_unit_scale_kernel(float* ts) {
+  griddep_wait();
+  *ts = 1.0f;
+}
+
+struct AmaxParams {
+  const void* x;
+  int64_t rows, cols, ld, segs;  // segs: 512-element segments per row
+  int32_t wide;
+  float* partials;
+};
+
+// WIDE: every row starts on 32 bytes. One 512-element segment per warp and step, four (two
+// of fp32) in flight.
+template <int DT, bool WIDE>
+__global__ void __launch_bounds__(256, 4) mx_amax_kernel(const AmaxParams p) {
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t per_row = (cols + 15) / 16;
-  const int64_t warps_per_row = (per_row + 31) / 32;
-  const int64_t tasks = rows * warps_per_row;
-  const uint32_t lane = lane_id();
-  uint32_t m = 0;
-  for (int64_t t = int64_t(blockIdx.x) * 8 + warp_id(); t < tasks; t += int64_t(gridDim.x) * 8) {
-    const int64_t row = t / warps_per_row;
-    const int64_t c = ((t - row * warps_per_row) * 32 + lane) * 16;
-    float v[16];
-    const int64_t left = cols - c;
-    load16<DT>(x + row * ld + c, wide && left >= 16, left < 16 ? int(left) : 16, v);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t b = abs_bits(v[i]);
-      m = max(m, b < 0x7F800000u ? b : 0u);
+  using T = typename Elem<DT>::T;
+  constexpr int FLY = WIDE ? (sizeof(T) == 2 ? 4 : 2) : 1;
+  __shared__ float stage[WIDE ? 1 : 8][kStageFloats];
+  __shared__ uint32_t red[8];
+  __shared__ uint32_t part[kAmaxCluster];
+  const T* x = static_cast<const T*>(p.x);
+  const int64_t tasks = p.rows * p.segs;
+  const uint32_t lane = lane_id(), warp = warp_id();
+  const int64_t step = int64_t(gridDim.x) * 8;
+  const auto segment = [&](int64_t t, Raw16<DT>& w) {
+    const int64_t row = p.rows == 1 ? 0 : t >> 32 ? t / p.segs : uint32_t(t) / uint32_t(p.segs);
+    const int64_t c0 = (t - row * p.segs) * 512, left = p.cols - c0;
+    const T* src = x + row * p.ld + c0;
+    if constexpr (WIDE) {
+      const int64_t n = left - 16 * int64_t(lane);
+      w.load(src + 16 * lane, n >= 16, n < 16 ? int(n) : 16);
+    } else {
+      warp_load16<DT>(src, left, stage[warp], w);
     }
+  };
+  uint32_t m = 0;
+  const auto fold = [&](const Raw16<DT>& w) {
+    const uint32_t a = amax_raw<DT>(w);
+    if (a < 0x7F800000u) {
+      m = max(m, a);
+    } else {  // rare: something in it does not count
+      float v[16];
+      w.unpack(v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t b = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+        if (b < 0x7F800000u) m = max(m, b);
+      }
+    }
+  };
+  int64_t t = int64_t(blockIdx.x) * 8 + warp;
+  for (; t + (FLY - 1) * step < tasks; t += FLY * step) {
+    Raw16<DT> w[FLY];
+#pragma unroll
+    for (int i = 0; i < FLY; ++i) segment(t + i * step, w[i]);
+#pragma unroll
+    for (int i = 0; i < FLY; ++i) fold(w[i]);
+  }
+  for (; t < tasks; t += step) {
+    Raw16<DT> w;
+    segment(t, w);
+    fold(w);
   }
   m = __reduce_max_sync(0xffffffffu, m);
-  __shared__ uint32_t red[8];
-  if (lane == 0) red[warp_id()] = m;
+  if (lane == 0) red[warp] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) m = max(m, red[i]);
-    atomicMax(ts + 1, m);
-    __threadfence();
-    if (atomicAdd(ts + 2, 1u) == gridDim.x - 1) {
-      __threadfence();
-      const float amax = __uint_as_float(atomicMax(ts + 1, 0u));
-      // kept normal so that its reciprocal is finite
-      *reinterpret_cast<float*>(ts) = amax > 0.0f ? fmaxf(__fdiv_rn(amax, 2688.0f), 1.17549435e-38f) : 1.0f;
-    }
+    st_shared_cluster_u32(mapa_shared(smem_u32(part + cluster_ctarank()), 0), m);
   }
+  cluster_sync();
+  if (cluster_ctarank() == 0 && threadIdx.x == 0) {
+    const uint32_t n = cluster_nctarank();
+    for (uint32_t i = 0; i < n; ++i) m = max(m, part[i]);
+    p.partials[blockIdx.x / n] = __uint_as_float(m);
+  }
+}
+
+// The tensor scale from `n` <= 64 partial maxima, in every lane of the warp; kept normal so
+// that its reciprocal is finite. Ordinary loads, here and of given tensor scales: an earlier
+// kernel of the stream may have written them after this one was launched, which the
+// read-only path does not allow for, and reading past L1 (every warp the same line of L2)
+// took 10 us of a 17 us launch at 2048 x 4096.
+__device__ __forceinline__ float tensor_scale_from(const float* partials, uint32_t n) {
+  const uint32_t lane = lane_id();
+  uint32_t m = lane < n ? __float_as_uint(partials[lane]) : 0u;
+  if (lane + 32 < n) m = max(m, __float_as_uint(partials[lane + 32]));
+  m = __reduce_max_sync(0xffffffffu, m);
+  return m ? fmaxf(__fdiv_rn(__uint_as_float(m), 2688.0f), 1.17549435e-38f) : 1.0f;
 }
 
 // ---------------------------------------------------------------------------------
@@ -74,117 +136,184 @@ struct QuantParams {
   int64_t rows, cols, ldx;  // of the quantised matrix (after the transposition, if any)
   uint8_t* data;
   uint8_t* scales;
-  const float* tensor_scale;  // may be null
-  int64_t ld;                 // bytes
+  float* tensor_scale;    // may be null
+  const float* partials;  // not null: find the tensor scale from these and store it
+  uint32_t n_partials;
+  int64_t ld;             // bytes
   int64_t groups;
   int32_t wide;
 };
 
-// One warp per 512 consecutive elements of a row; rows run on to a multiple of 128 so
-// that the padding bytes of the last scale tiles are written (as zero).
-template <int FMT, int DT>
+// Reciprocal of the tensor scale that an NV_FP4 quantiser works with (1 without one).
+__device__ __forceinline__ float scale_reciprocal(const QuantParams& p) {
+  if (p.partials) {
+    const float ts = tensor_scale_from(p.partials, p.n_partials);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.tensor_scale = ts;
+    return __frcp_rn(ts);
+  }
+  return p.tensor_scale ? __frcp_rn(*p.tensor_scale) : 1.0f;
+}
+
+// One warp per CH segments of 512 consecutive elements of a row; rows run on to a multiple
+// of 128 so that the padding bytes of the last scale tiles are written (as zero). WIDE:
+// every row starts on 32 bytes.
+template <int FMT, int DT, int CH, bool WIDE>
 __global__ void __launch_bounds__(256) mx_quant_rows_kernel(const QuantParams p) {
   griddep_wait();
   griddep_launch_dependents();
   using T = typename Elem<DT>::T;
-  const int64_t warps_per_row = (p.groups * 4 * MxFmt<FMT>::BLOCK + 511) / 512;
-  const int64_t t = int64_t(blockIdx.x) * 8 + warp_id();
-  const int64_t row = t / warps_per_row;
+  __shared__ float stage[WIDE ? 1 : 8][kStageFloats];
+  const uint32_t lane = lane_id(), warp = warp_id();
+  const uint32_t warps_per_row = uint32_t((p.groups * 4 * MxFmt<FMT>::BLOCK + 512 * CH - 1) / (512 * CH));
+  const int64_t t = int64_t(blockIdx.x) * 8 + warp;
+  const int64_t row = t >> 32 ? t / warps_per_row : uint32_t(t) / warps_per_row;
   if (row >= (p.rows + 127) / 128 * 128) return;  // whole warps
-  const uint32_t lane = lane_id();
-  const int64_t c = ((t - row * warps_per_row) * 32 + lane) * 16;
-  float v[16];
-  const int64_t left = row < p.rows ? p.cols - c : 0;
-  load16<DT>(static_cast<const T*>(p.x) + row * p.ldx + c, p.wide && left >= 16, left < 16 ? int(left) : 16, v);
-  if constexpr (FMT == NV_FP4) {
-    if (p.tensor_scale) {
-      const float r = __frcp_rn(__ldg(p.tensor_scale));
+  const int64_t c0 = (t - row * warps_per_row) * (512 * CH);
+  const T* src = static_cast<const T*>(p.x) + row * p.ldx + c0;
+  Raw16<DT> w[CH];
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch) {
+    const int64_t left = row < p.rows ? p.cols - c0 - 512 * ch : 0;
+    if constexpr (WIDE) {
+      const int64_t n = left - 16 * int64_t(lane);
+      w[ch].load(src + 512 * ch + 16 * lane, n >= 16, n < 16 ? int(n) : 16);
+    } else {
+      warp_load16<DT>(src + 512 * ch, left, stage[warp], w[ch]);
+    }
+  }
+  float r = 1.0f;
+  if constexpr (FMT == NV_FP4) r = scale_reciprocal(p);
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch) {
+    const int64_t c = c0 + 512 * ch + 16 * lane;
+    uint32_t amax = amax_raw<DT>(w[ch]);
+    float v[16];
+    w[ch].unpack(v);
+    if constexpr (FMT == NV_FP4) {  // r > 0 and rounding are monotone: the largest stays the largest
+      amax = __float_as_uint(__uint_as_float(amax) * r);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] *= r;
     }
-  }
-  uint32_t q[4];
-  const uint32_t word = mx_gather_scales<FMT>(mx_quantize16<FMT>(v, q));
-  const int64_t g = c / (4 * MxFmt<FMT>::BLOCK);
-  if (lane % kLanesPerGroup<FMT> == 0 && g < p.groups)
-    *reinterpret_cast<uint32_t*>(p.scales + mx_scale_word(row, g, p.groups)) = word;
-  if (row < p.rows && c < mx_padded_cols(p.cols)) {
-    uint8_t* d = p.data + row * p.ld + c * MxFmt<FMT>::BITS / 8;
-    if constexpr (FMT == MX_FP8) *reinterpret_cast<uint4*>(d) = make_uint4(q[0], q[1], q[2], q[3]);
-    else *reinterpret_cast<uint2*>(d) = make_uint2(q[0], q[1]);
+    uint32_t q[4];
+    const uint32_t word = mx_gather_scales<FMT>(mx_quantize16<FMT>(v, amax, q));
+    const int64_t g = c / (4 * MxFmt<FMT>::BLOCK);
+    if (lane % kLanesPerGroup<FMT> == 0 && g < p.groups)
+      *reinterpret_cast<uint32_t*>(p.scales + mx_scale_word(row, g, p.groups)) = word;
+    if (row < p.rows && c < mx_padded_cols(p.cols)) {
+      uint8_t* d = p.data + row * p.ld + c * MxFmt<FMT>::BITS / 8;
+      if constexpr (FMT == MX_FP8) *reinterpret_cast<uint4*>(d) = make_uint4(q[0], q[1], q[2], q[3]);
+      else *reinterpret_cast<uint2*>(d) = make_uint2(q[0], q[1]);
+    }
   }
 }
 
 // ---------------------------------------------------------------------------------
 // quantise along the columns of x: q = quantise(x^T)
 // ---------------------------------------------------------------------------------
-// A CTA takes 128 rows (k) x 64 columns of x through shared memory. Thread t then owns
-// output rows (columns of x) 2p, 2p + 1 and a 32-long piece s of k: lane = 8 pairs x 4
-// pieces, so four lanes write 128 (64) consecutive bytes of one output row. Column pairs
-// are stored at p ^ (8 * piece), so the four pieces' reads of one step fall into
-// different banks.
+// A CTA takes 128 rows (k) x 64 columns of x through shared memory. A thread then owns two
+// output rows (columns of x) and a 32-long piece of k: lane = 8 columns or column pairs x 4
+// pieces, so four lanes write 128 (64) consecutive bytes of one output row. 16-bit types are
+// read as pairs of neighbouring columns, fp32 as single ones 32 apart; both sit flipped by
+// 8 * piece (in pairs or columns), so the four pieces' reads fall into different banks.
+template <int DT>
+struct ColsTile {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  static constexpr bool PAIRS = sizeof(T) == 2;
+  static constexpr int VEC = 16 / sizeof(T);  // elements per 16-byte access
+  // place of column c in a tile row of piece s (a 16-byte vector never straddles a flip)
+  static __device__ __forceinline__ int place(int c, int s) { return c ^ (PAIRS ? 16 * s : 8 * s); }
+};
+
 template <int FMT, int DT>
 __global__ void __launch_bounds__(128) mx_quant_cols_kernel(const QuantParams p) {
   griddep_wait();
   griddep_launch_dependents();
+  using Tile = ColsTile<DT>;
   using E = Elem<DT>;
   using T = typename E::T;
-  constexpr int kVec = 16 / sizeof(T);  // elements per 16-byte load
+  constexpr int kVec = Tile::VEC;
   __shared__ alignas(16) T tile[128][64];
+  float r = 1.0f;
+  if constexpr (FMT == NV_FP4) r = scale_reciprocal(p);
   const uint32_t strips = uint32_t((p.rows + 127) / 128 * 2);
   const int64_t k0 = int64_t(blockIdx.x / strips) * 128;  // x row
   const int64_t c0 = int64_t(blockIdx.x % strips) * 64;   // x column = output row
   const T* x = static_cast<const T*>(p.x);
   const int64_t kleft = p.cols - k0, cleft = p.rows - c0;
-  // element (k, c) sits at [k][((c / 2) ^ (8 * (k / 32))) * 2 + c % 2]
   if (p.wide) {
     constexpr int kPerRow = 64 / kVec;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < 128 * kPerRow; i += 128) {
-      const int k = i / kPerRow, c = i % kPerRow * kVec;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (k < kleft) {
-        const T* src = x + (k0 + k) * p.ldx + c0 + c;
-        if (c + kVec <= cleft) {
-          w = *reinterpret_cast<const uint4*>(src);
-        } else if (c < cleft) {
-          alignas(16) T e[kVec];
+    constexpr int kLoads = 128 * kPerRow / 128;  // per thread: 8 or 16, eight in flight
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) e[j] = c + j < cleft ? src[j] : E::store(0.0f);
-          w = *reinterpret_cast<const uint4*>(e);
+    for (int b = 0; b < kLoads; b += 8) {
+      uint4 w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = (b + j) * 128 + threadIdx.x, k = i / kPerRow, c = i % kPerRow * kVec;
+        w[j] = make_uint4(0, 0, 0, 0);
+        if (k < kleft && c < cleft) {
+          const T* src = x + (k0 + k) * p.ldx + c0 + c;
+          if (c + kVec <= cleft) {
+            w[j] = __ldcs(reinterpret_cast<const uint4*>(src));
+          } else {
+            alignas(16) T e[kVec];
+#pragma unroll
+            for (int l = 0; l < kVec; ++l) e[l] = c + l < cleft ? src[l] : E::store(0.0f);
+            w[j] = *reinterpret_cast<const uint4*>(e);
+          }
         }
       }
-      // a 16-byte vector holds 4 or 2 pairs and the flip moves groups of 8 pairs
-      *reinterpret_cast<uint4*>(&tile[k][((c / 2) ^ (8 * (k / 32))) * 2]) = w;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = (b + j) * 128 + threadIdx.x, k = i / kPerRow, c = i % kPerRow * kVec;
+        *reinterpret_cast<uint4*>(&tile[k][Tile::place(c, k / 32)]) = w[j];
+      }
     }
   } else {
+#pragma unroll 8
     for (int i = threadIdx.x; i < 128 * 64; i += 128) {
       const int k = i / 64, c = i % 64;
-      tile[k][((c / 2) ^ (8 * (k / 32))) * 2 + c % 2] =
-          k < kleft && c < cleft ? x[(k0 + k) * p.ldx + c0 + c] : E::store(0.0f);
+      tile[k][Tile::place(c, k / 32)] = k < kleft && c < cleft ? x[(k0 + k) * p.ldx + c0 + c] : E::store(0.0f);
     }
   }
   __syncthreads();
   const uint32_t lane = lane_id();
-  const int piece = lane & 3, pair = warp_id() * 8 + (lane >> 2);
-  const int col = (pair ^ (8 * piece)) * 2;
-  float r = 1.0f;
-  if constexpr (FMT == NV_FP4)
-    if (p.tensor_scale) r = __frcp_rn(__ldg(p.tensor_scale));
+  const int piece = lane & 3, slot = warp_id() * 8 + (lane >> 2);
+  constexpr int NB = 32 / MxFmt<FMT>::BLOCK;
+  uint32_t pairs[Tile::PAIRS ? 32 : 1], two[NB];  // two: both columns' block maxima
+  if constexpr (Tile::PAIRS) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      pairs[i] = *reinterpret_cast<const uint32_t*>(&tile[32 * piece + i][Tile::place(2 * slot, piece)]);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) two[b] = amax_packed<32 / NB>(pairs + b * (32 / NB));
+  }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int64_t row = c0 + 2 * pair + h;  // output row
-    uint32_t amax = 0, byte[2];
+    const int col = Tile::PAIRS ? 2 * slot + h : slot + 32 * h;
+    const int64_t row = c0 + col;  // output row
+    uint32_t byte[2];
     uint32_t q[8];
     float v[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = E::load(tile[32 * piece + i][col + h]) * r;
-    constexpr int NB = 32 / MxFmt<FMT>::BLOCK;
+    for (int i = 0; i < 32; ++i) {
+      if constexpr (Tile::PAIRS) {
+        const float2 f = E::unpack(pairs[i]);
+        v[i] = h ? f.y : f.x;
+      } else {
+        v[i] = tile[32 * piece + i][Tile::place(col, piece)];
+      }
+      if constexpr (FMT == NV_FP4) v[i] *= r;
+    }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      amax = 0;
-#pragma unroll
-      for (int i = 0; i < 32 / NB; ++i) amax = max(amax, abs_bits(v[b * (32 / NB) + i]));
+      uint32_t amax;
+      if constexpr (Tile::PAIRS) {
+        amax = widen_bits<DT>(h ? two[b] >> 16 : two[b]);
+        if constexpr (FMT == NV_FP4) amax = __float_as_uint(__uint_as_float(amax) * r);
+      } else {
+        amax = amax_bits<32 / NB>(v + b * (32 / NB));
+      }
       if constexpr (FMT == NV_FP4) {
         byte[b] = nv_scale_byte(amax);
         const NvInverse inv(byte[b]);
@@ -245,21 +374,23 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
   return byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u);  // 2^-127 is subnormal
 }
 
-template <int FMT, int DT>
+template <int FMT, int DT, bool WIDE>
 __global__ void __launch_bounds__(256) mx_dequant_kernel(const DequantParams p) {
   griddep_wait();
   griddep_launch_dependents();
   using T = typename Elem<DT>::T;
-  const int64_t warps_per_row = (p.cols + 511) / 512;
+  __shared__ float stage[WIDE ? 1 : 8][kStageFloats];
+  const uint32_t warps_per_row = uint32_t((p.cols + 511) / 512);
   const int64_t t = int64_t(blockIdx.x) * 8 + warp_id();
-  const int64_t row = t / warps_per_row;
-  if (row >= p.rows) return;
-  const int64_t c = ((t - row * warps_per_row) * 32 + lane_id()) * 16;
-  if (c >= p.cols) return;
+  const int64_t row = t >> 32 ? t / warps_per_row : uint32_t(t) / warps_per_row;
+  if (row >= p.rows) return;  // whole warps
+  const int64_t c0 = (t - row * warps_per_row) * 512;
+  const bool mine = c0 + 16 * int64_t(lane_id()) < p.cols;
+  const int64_t c = mine ? c0 + 16 * lane_id() : c0;  // lanes behind the row repeat its first chunk
   const uint8_t* d = p.data + row * p.ld + c * MxFmt<FMT>::BITS / 8;
   const int64_t b = c / MxFmt<FMT>::BLOCK;
-  float s = mx_scale_value<FMT>(__ldg(p.scales + mx_scale_word(row, b / 4, p.groups) + (b & 3)));
-  const float ts = (FMT == NV_FP4 && p.tensor_scale) ? __ldg(p.tensor_scale) : 1.0f;
+  float s = mx_scale_value<FMT>(p.scales[mx_scale_word(row, b / 4, p.groups) + (b & 3)]);
+  const float ts = (FMT == NV_FP4 && p.tensor_scale) ? *p.tensor_scale : 1.0f;
   float v[16];
   if constexpr (FMT == MX_FP8) {
     const uint4 w = *reinterpret_cast<const uint4*>(d);
@@ -290,8 +421,12 @@ __global__ void __launch_bounds__(256) mx_dequant_kernel(const DequantParams p) 
       v[2 * i + 1] = f.y * s * ts;
     }
   }
-  const int64_t left = p.cols - c;
-  store16<DT>(static_cast<T*>(p.y) + row * p.ldy + c, p.wide && left >= 16, left < 16 ? int(left) : 16, v);
+  if constexpr (WIDE) {
+    const int64_t left = mine ? p.cols - c : 0;
+    store16<DT>(static_cast<T*>(p.y) + row * p.ldy + c, left >= 16, left < 16 ? int(left) : 16, v);
+  } else {
+    warp_store16<DT>(static_cast<T*>(p.y) + row * p.ldy + c0, p.cols - c0, stage[warp_id()], v);
+  }
 }
 
 // ---------------------------------------------------------------------------------
@@ -308,15 +443,96 @@ struct NormParams {
   uint8_t* scales;
   const float* tensor_scale;
   int64_t ld, groups;
-  int32_t wide, weight_f32;
+  int32_t wide, wide_weight, weight_f32, stream;
+  uint32_t* status;
+  uint64_t wait_ns;
 };
 
-// TR threads per row, CH chunks of 16 elements per thread: the whole row stays in
-// registers between the sum of squares and the quantisation, so every tensor is read or
-// written once. x + residual is kept unrounded in fp32 for the norm; h is its one
-// rounding. A row's h is written before its thread has anything to read again, so h may
-// be x or residual itself.
-template <int FMT, int DT, int TR, int CH>
+// x + residual is kept unrounded in fp32 for the norm; h is its one rounding. The whole row
+// stays in registers between the sum of squares and the quantisation, so every tensor is
+// read or written once.
+//
+// 16 consecutive elements of a row in shared memory (16-byte aligned), n of which exist; a
+// row's length is a multiple of 16 bytes.
+template <int DT>
+__device__ __forceinline__ void norm_read16(const uint8_t* a, int n, float (&v)[16]) {
+  using E = Elem<DT>;
+  constexpr int PER = 16 / sizeof(typename E::T);
+#pragma unroll
+  for (int j = 0; j < 16 / PER; ++j) {
+    const uint4 w = j * PER < n ? reinterpret_cast<const uint4*>(a)[j] : make_uint4(0, 0, 0, 0);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (PER == 8) {
+        const float2 f = E::unpack(u[i]);
+        v[8 * j + 2 * i] = f.x;
+        v[8 * j + 2 * i + 1] = f.y;
+      } else {
+        v[4 * j + i] = __uint_as_float(u[i]);
+      }
+    }
+  }
+}
+
+// The last part of both kernels: one 16-element chunk at column c of row `row`, of which n
+// elements exist, from h in fp32 to elements and scales. Elements behind the last column and
+// rows behind the last are zero even where the row's norm is NaN. Whole warps, 512 columns.
+//
+// y = h * rstd * w is held in 32 bits as z = h * w and the row's factor: the block's largest
+// |y| is rstd * max|z|, and the element is z times one factor, rstd over the block scale.
+// That is two multiplications per element where y, its scaling and (NV_FP4) a correctly
+// rounded quotient took up to seven; y is rounded arithmetic either way, so nothing hangs on
+// a tie. `rstd` includes the reciprocal tensor scale.
+template <int FMT>
+__device__ __forceinline__ void norm_store(const NormParams& p, int64_t row, bool live, int c, int n, float rstd,
+                                           const float (&w)[16], float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] *= w[i];
+  if (n < 16) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i >= n) v[i] = 0.0f;
+  }
+  uint32_t amax = amax_bits<16>(v);
+  if constexpr (MxFmt<FMT>::BLOCK == 32) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  // an all-zero block stays zero whatever the factor is (rstd may be infinite or NaN only
+  // where the row itself is not finite)
+  const uint32_t ymax = amax ? __float_as_uint(__uint_as_float(amax) * rstd) & 0x7FFFFFFFu : 0u;
+  uint32_t byte;
+  float f;
+  if constexpr (FMT == NV_FP4) {
+    byte = nv_scale_byte(ymax);
+    f = rstd * NvInverse(byte).r;
+  } else {
+    byte = mx_scale_byte<FMT>(ymax);
+    f = rstd * mx_inverse_scale(byte);
+    if (byte < 32) {  // |y| below 2^-90: the factor alone could overflow
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] *= rstd;
+      f = mx_inverse_scale(byte);
+    }
+  }
+  if (amax == 0) f = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] *= f;
+  uint32_t q[4];
+  mx_pack16<FMT>(v, q);
+  const uint32_t word = mx_gather_scales<FMT>(byte);
+  const int g = c / (4 * MxFmt<FMT>::BLOCK);
+  if (lane_id() % kLanesPerGroup<FMT> == 0 && g < p.groups && row < (p.rows + 127) / 128 * 128)
+    *reinterpret_cast<uint32_t*>(p.scales + mx_scale_word(row, g, p.groups)) = word;
+  if (live && c < mx_padded_cols(p.cols)) {
+    uint8_t* d = p.data + row * p.ld + c * MxFmt<FMT>::BITS / 8;
+    if constexpr (FMT == MX_FP8) *reinterpret_cast<uint4*>(d) = make_uint4(q[0], q[1], q[2], q[3]);
+    else *reinterpret_cast<uint2*>(d) = make_uint2(q[0], q[1]);
+  }
+}
+
+// mx_rms_norm_kernel: TR threads per row, CH chunks of 16 elements per thread. A thread has
+// read its chunk of x and residual before it writes that chunk of h, and no other thread
+// reads it, so h may be x or residual itself.
+template <int FMT, int DT, int TR, int CH, bool WIDE>
 __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const NormParams p) {
   griddep_wait();
   griddep_launch_dependents();
@@ -324,24 +540,31 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
   constexpr int NT = TR < 256 ? 256 : TR;
   constexpr int ROWS = NT / TR;       // rows per CTA
   constexpr int WARPS = TR / 32;      // warps per row
+  __shared__ float stage[WIDE ? 1 : NT / 32][kStageFloats];
   const int r_in = threadIdx.x / TR, t = threadIdx.x % TR;
+  const uint32_t warp = warp_id(), lane = lane_id();
   const int64_t row = int64_t(blockIdx.x) * ROWS + r_in;
   const bool live = row < p.rows;     // rows behind the last only write zero scales
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   float v[CH][16];
   float ss = 0.0f;
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
-    const int64_t c = int64_t(ch * TR + t) * 16;
-    const int64_t left = live ? p.cols - c : 0;
-    const int n = left < 16 ? (left < 0 ? 0 : int(left)) : 16;
-    const bool wide = p.wide && n == 16;
-    load16<DT>(static_cast<const T*>(p.x) + row * p.ldx + c, wide, n, v[ch]);
+    const int c = (ch * TR + t) * 16, wc = c - 16 * int(lane);  // this thread's column, its warp's
+    const int warp_left = live ? int(p.cols) - wc : 0;
+    const int n = min(16, max(0, warp_left - 16 * int(lane)));
+    if constexpr (WIDE) load16<DT>(x + c, n == 16, n, v[ch]);
+    else warp_load16<DT>(x + wc, warp_left, stage[warp], v[ch]);
     if (p.residual) {
+      const T* res = static_cast<const T*>(p.residual) + row * p.ldr;
+      T* h = static_cast<T*>(p.h) + row * p.ldh;
       float r[16];
-      load16<DT>(static_cast<const T*>(p.residual) + row * p.ldr + c, wide, n, r);
+      if constexpr (WIDE) load16<DT>(res + c, n == 16, n, r);
+      else warp_load16<DT>(res + wc, warp_left, stage[warp], r);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[ch][i] += r[i];
-      store16<DT>(static_cast<T*>(p.h) + row * p.ldh + c, wide, n, v[ch]);
+      if constexpr (WIDE) store16<DT>(h + c, n == 16, n, v[ch]);
+      else warp_store16<DT>(h + wc, warp_left, stage[warp], v[ch]);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) ss = fmaf(v[ch][i], v[ch][i], ss);
@@ -350,51 +573,141 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   if constexpr (WARPS > 1) {
     __shared__ float red[NT / 32];
-    if (lane_id() == 0) red[warp_id()] = ss;
+    if (lane == 0) red[warp] = ss;
     __syncthreads();
     const float* mine = red + r_in * WARPS;
     ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) ss += mine[i];
   }
-  const float rstd = rsqrtf(fmaf(ss, p.inv_cols, p.eps));
-  float pre = 1.0f;
+  float rstd = rsqrtf(fmaf(ss, p.inv_cols, p.eps));
   if constexpr (FMT == NV_FP4)
-    if (p.tensor_scale) pre = __frcp_rn(__ldg(p.tensor_scale));
+    if (p.tensor_scale) rstd *= __frcp_rn(*p.tensor_scale);
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
-    const int64_t c = int64_t(ch * TR + t) * 16;
-    const int64_t left = live ? p.cols - c : 0;
-    const int n = left < 16 ? (left < 0 ? 0 : int(left)) : 16;
+    const int c = (ch * TR + t) * 16;
+    if (c - 16 * int(lane) >= p.groups * (4 * MxFmt<FMT>::BLOCK)) continue;  // the whole warp is behind the row
+    const int n = min(16, max(0, live ? int(p.cols) - c : 0));
     float w[16];
-    if (p.weight_f32) load16<3>(static_cast<const float*>(p.weight) + c, p.wide && n == 16, n, w);
-    else load16<DT>(static_cast<const T*>(p.weight) + c, p.wide && n == 16, n, w);
+    if (p.weight_f32) load16<3, true>(static_cast<const float*>(p.weight) + c, p.wide_weight && n == 16, n, w);
+    else load16<DT, true>(static_cast<const T*>(p.weight) + c, p.wide_weight && n == 16, n, w);
+    norm_store<FMT>(p, row, live, c, n, rstd, w, v[ch]);
+  }
+}
+
+// mx_rms_norm_stream_kernel: many rows. The kernel above keeps as many bytes in flight as
+// its threads hold in registers, 32 or 64 each, and stops loading while a row is reduced and
+// stored (8192 x 8192 bf16: 112 us with a residual, 83 without; the bytes alone: 73 and 31).
+// Here a CTA takes rows r, r + grid, ... and one thread copies whole rows of x and residual
+// into a ring in shared memory with cp.async.bulk, kNormStages rows ahead, so the loads of
+// the next rows run under everything else. NT threads, CH chunks each. Rows start on 16
+// bytes and are a multiple of 16 bytes long. A row of h is written after its row of x and
+// residual was read whole, so h may again be either of them.
+constexpr int kNormStages = 3;
+
+template <int FMT, int DT, int NT, int CH>
+__global__ void __launch_bounds__(NT) mx_rms_norm_stream_kernel(const NormParams p) {
+  using T = typename Elem<DT>::T;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float red[2][NT / 32];
+  __shared__ __align__(8) uint64_t full[kNormStages];
+  const uint32_t warp = warp_id(), lane = lane_id();
+  const uint32_t row_bytes = uint32_t(p.cols * sizeof(T));
+  const uint32_t stage_bytes = row_bytes * (p.residual ? 2 : 1);
+  if (threadIdx.x == 0) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float y = v[ch][i] * rstd * w[i];
-      if constexpr (FMT == NV_FP4) y *= pre;
-      v[ch][i] = y;
+    for (int s = 0; s < kNormStages; ++s) mbar_init(smem_u32(full + s), 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  griddep_wait();
+  griddep_launch_dependents();
+  const T* x = static_cast<const T*>(p.x);
+  const T* res = static_cast<const T*>(p.residual);
+  const auto load_row = [&](int64_t row, int s) {
+    const uint32_t bar = smem_u32(full + s), dst = smem_u32(smem) + s * stage_bytes;
+    mbar_arrive_expect_tx(bar, stage_bytes);
+    bulk_load(dst, x + row * p.ldx, row_bytes, bar);
+    if (res) bulk_load(dst + row_bytes, res + row * p.ldr, row_bytes, bar);
+  };
+  const int64_t first = blockIdx.x, step = gridDim.x;
+  if (threadIdx.x == 0)
+    for (int s = 0; s < kNormStages; ++s)
+      if (first + s * step < p.rows) load_row(first + s * step, s);
+  float pre = 1.0f;
+  if constexpr (FMT == NV_FP4)
+    if (p.tensor_scale) pre = __frcp_rn(*p.tensor_scale);
+
+  int s = 0;
+  uint32_t phase = 0, parity = 0;
+  bool ok = true;
+  for (int64_t row = first; row < p.rows; row += step) {
+    // all threads wait; a wait that runs out ends this CTA's work (status word)
+    ok = mbar_wait_bounded(smem_u32(full + s), phase, p.wait_ns);
+    const uint8_t* sx = smem + s * stage_bytes;
+    float v[CH][16];
+    float ss = 0.0f;
+    T* h = static_cast<T*>(p.h) + row * p.ldh;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      const int c = (ch * NT + threadIdx.x) * 16;
+      const int n = min(16, max(0, int(p.cols) - c));
+      if (c - 16 * int(lane) >= int(p.cols)) {  // the whole warp is behind the row
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[ch][i] = 0.0f;
+        continue;
+      }
+      norm_read16<DT>(sx + c * sizeof(T), n, v[ch]);
+      if (res) {
+        float r[16];
+        norm_read16<DT>(sx + row_bytes + c * sizeof(T), n, r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[ch][i] += r[i];
+        store16<DT>(h + c, p.wide && n == 16, n, v[ch]);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ss = fmaf(v[ch][i], v[ch][i], ss);
     }
-    if (live) {
-      // elements behind the last column: zero even where the row's norm is NaN
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i >= n) v[ch][i] = 0.0f;
-    } else {
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (lane == 0) red[parity][warp] = ss;
+    ok = __syncthreads_and(ok);
+    if (!ok) break;
+    // every thread has read the stage: refill it
+    if (threadIdx.x == 0 && row + kNormStages * step < p.rows) load_row(row + kNormStages * step, s);
+    ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[ch][i] = 0.0f;
+    for (int i = 0; i < NT / 32; ++i) ss += red[parity][i];
+    parity ^= 1u;  // the other buffer: a fast warp's next sum must not overtake a slow one's read
+    const float rstd = rsqrtf(fmaf(ss, p.inv_cols, p.eps)) * pre;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+      const int c = (ch * NT + threadIdx.x) * 16;
+      const int n = min(16, max(0, int(p.cols) - c));
+      if (c - 16 * int(lane) >= p.groups * (4 * MxFmt<FMT>::BLOCK)) continue;
+      float w[16];
+      if (p.weight_f32) load16<3, true>(static_cast<const float*>(p.weight) + c, p.wide_weight && n == 16, n, w);
+      else load16<DT, true>(static_cast<const T*>(p.weight) + c, p.wide_weight && n == 16, n, w);
+      norm_store<FMT>(p, row, true, c, n, rstd, w, v[ch]);
     }
-    uint32_t q[4];
-    const uint32_t word = mx_gather_scales<FMT>(mx_quantize16<FMT>(v[ch], q));
-    const int64_t g = c / (4 * MxFmt<FMT>::BLOCK);
-    if (t % kLanesPerGroup<FMT> == 0 && g < p.groups && row < (p.rows + 127) / 128 * 128)
-      *reinterpret_cast<uint32_t*>(p.scales + mx_scale_word(row, g, p.groups)) = word;
-    if (live && c < mx_padded_cols(p.cols)) {
-      uint8_t* d = p.data + row * p.ld + c * MxFmt<FMT>::BITS / 8;
-      if constexpr (FMT == MX_FP8) *reinterpret_cast<uint4*>(d) = make_uint4(q[0], q[1], q[2], q[3]);
-      else *reinterpret_cast<uint2*>(d) = make_uint2(q[0], q[1]);
+    if (++s == kNormStages) {
+      s = 0;
+      phase ^= 1u;
     }
   }
+  if (!ok) {
+    // a copy never landed: report it, and wait once more for those in flight before the
+    // shared memory goes away
+    if (threadIdx.x == 0) {
+      if (p.status) atomicOr(p.status, ST_PRODUCER_EMPTY | ST_ABORTED);
+      for (int i = 0; i < kNormStages; ++i) (void)mbar_wait_bounded(smem_u32(full + i), i < s ? phase ^ 1u : phase, p.wait_ns);
+    }
+    __syncthreads();
+  }
+  // zero scales of the rows behind the last one
+  const int64_t end = (p.rows + 127) / 128 * 128;
+  for (int64_t i = int64_t(blockIdx.x) * NT + threadIdx.x; i < (end - p.rows) * p.groups; i += step * NT)
+    *reinterpret_cast<uint32_t*>(p.scales + mx_scale_word(p.rows + i / p.groups, i % p.groups, p.groups)) = 0u;
 }
 
 // ---------------------------------------------------------------------------------
@@ -403,16 +716,22 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
 // Programmatic dependent launch, as the GEMM's: every kernel here waits
 // (griddepcontrol.wait) before its first global access.
 template <typename P>
-int launch(void (*kern)(P), dim3 grid, unsigned threads, const P& p, cudaStream_t stream) {
+int launch(void (*kern)(P), dim3 grid, unsigned threads, unsigned cluster, const P& p, cudaStream_t stream,
+           size_t smem = 0) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) {
     (void)cudaGetLastError();
     return B200_ERR_LAUNCH;
@@ -424,40 +743,54 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 int elem_size(int dt) { return dt == B200_DT_F32 ? 4 : (dt == B200_DT_F16 || dt == B200_DT_BF16) ? 2 : 0; }
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int kNormSmem = 220 * 1024;  // of a streaming CTA's rows
 
 template <int FMT, int DT>
-int quantize_t(QuantParams p, bool transpose, cudaStream_t s) {
+int quantize_t(const QuantParams& p, bool transpose, int sms, cudaStream_t s) {
   if (!transpose) {
-    const int64_t warps = (p.rows + 127) / 128 * 128 * ((p.groups * 4 * MxFmt<FMT>::BLOCK + 511) / 512);
-    const int64_t grid = (warps + 7) / 8;
+    // Two segments per warp for 16-bit types, 64 bytes in flight per thread (8192 x 8192
+    // bf16: MX_FP8 34.6 -> 33.2 us, NV_FP4 44.4 -> 38.4; fp32 has 64 with one), unless that
+    // leaves SMs without their 64 warps.
+    const int64_t rows = (p.rows + 127) / 128 * 128, segs = (p.groups * 4 * MxFmt<FMT>::BLOCK + 511) / 512;
+    const bool two = p.wide && DT != B200_DT_F32 && segs > 1 && rows * segs >= int64_t(sms) * 64;
+    const int64_t grid = (rows * (two ? (segs + 1) / 2 : segs) + 7) / 8;
     if (grid > kMaxGrid) return B200_ERR_SHAPE;
-    return launch(mx_quant_rows_kernel<FMT, DT>, dim3(unsigned(grid)), 256, p, s);
+    const dim3 g{unsigned(grid)};
+    if (!p.wide) return launch(mx_quant_rows_kernel<FMT, DT, 1, false>, g, 256, 1, p, s);
+    if constexpr (DT != B200_DT_F32)
+      if (two) return launch(mx_quant_rows_kernel<FMT, DT, 2, true>, g, 256, 1, p, s);
+    return launch(mx_quant_rows_kernel<FMT, DT, 1, true>, g, 256, 1, p, s);
   }
   const int64_t grid = ((p.rows + 127) / 128 * 2) * ((p.cols + 127) / 128);
   if (grid > kMaxGrid) return B200_ERR_SHAPE;
-  return launch(mx_quant_cols_kernel<FMT, DT>, dim3(unsigned(grid)), 128, p, s);
+  return launch(mx_quant_cols_kernel<FMT, DT>, dim3(unsigned(grid)), 128, 1, p, s);
 }
 
 template <int FMT>
-int quantize_f(int dt, const QuantParams& p, bool transpose, cudaStream_t s) {
+int quantize_f(int dt, const QuantParams& p, bool transpose, int sms, cudaStream_t s) {
   switch (dt) {
-    case B200_DT_F16: return quantize_t<FMT, 0>(p, transpose, s);
-    case B200_DT_BF16: return quantize_t<FMT, 1>(p, transpose, s);
-    default: return quantize_t<FMT, 3>(p, transpose, s);
+    case B200_DT_F16: return quantize_t<FMT, 0>(p, transpose, sms, s);
+    case B200_DT_BF16: return quantize_t<FMT, 1>(p, transpose, sms, s);
+    default: return quantize_t<FMT, 3>(p, transpose, sms, s);
   }
 }
 
 template <int DT>
-int amax_t(const void* x, int64_t rows, int64_t cols, int64_t ld, int wide, float* ts, int sms, cudaStream_t s) {
-  if (cudaMemsetAsync(ts, 0, 16, s) != cudaSuccess) return B200_ERR_CUDA;
-  const int64_t warps = rows * (((cols + 15) / 16 + 31) / 32);
-  int64_t grid = (warps + 7) / 8;
-  if (grid > int64_t(sms) * 8) grid = int64_t(sms) * 8;
-  if (grid < 1) grid = 1;
-  // a memset precedes, so an ordinary launch
-  mx_amax_kernel<DT><<<unsigned(grid), 256, 0, s>>>(static_cast<const typename Elem<DT>::T*>(x), rows, cols, ld, wide,
-                                                    reinterpret_cast<uint32_t*>(ts));
-  return cudaGetLastError() == cudaSuccess ? B200_OK : B200_ERR_LAUNCH;
+int amax_t(AmaxParams p, uint32_t* n_partials, cudaStream_t s) {
+  if (p.ld == p.cols && p.rows < (int64_t(1) << 62) / p.cols) {
+    p.cols *= p.rows;  // no gaps between the rows: one long row
+    p.rows = 1;
+  }
+  p.segs = (p.cols + 511) / 512;
+  // clusters of 8 CTAs, about two segments to a warp and at most kPartials clusters; a
+  // matrix of one CTA's size stays with one
+  const int64_t ctas = (p.rows * p.segs + 15) / 16;
+  const unsigned cluster = ctas < kAmaxCluster ? 1 : kAmaxCluster;
+  int64_t n = ctas < kAmaxCluster ? ctas : (ctas + kAmaxCluster - 1) / kAmaxCluster;
+  if (n > kPartials) n = kPartials;
+  *n_partials = uint32_t(n);
+  return launch(p.wide ? mx_amax_kernel<DT, true> : mx_amax_kernel<DT, false>, dim3(unsigned(n) * cluster), 256,
+                cluster, p, s);
 }
 
 template <int FMT>
@@ -465,10 +798,11 @@ int dequantize_f(int dt, const DequantParams& p, cudaStream_t s) {
   const int64_t grid = (p.rows * ((p.cols + 511) / 512) + 7) / 8;
   if (grid > kMaxGrid) return B200_ERR_SHAPE;
   const dim3 g{unsigned(grid)};
+  const auto go = [&](auto wide, auto any) { return p.wide ? launch(wide, g, 256, 1, p, s) : launch(any, g, 256, 1, p, s); };
   switch (dt) {
-    case B200_DT_F16: return launch(mx_dequant_kernel<FMT, 0>, g, 256, p, s);
-    case B200_DT_BF16: return launch(mx_dequant_kernel<FMT, 1>, g, 256, p, s);
-    default: return launch(mx_dequant_kernel<FMT, 3>, g, 256, p, s);
+    case B200_DT_F16: return go(mx_dequant_kernel<FMT, 0, true>, mx_dequant_kernel<FMT, 0, false>);
+    case B200_DT_BF16: return go(mx_dequant_kernel<FMT, 1, true>, mx_dequant_kernel<FMT, 1, false>);
+    default: return go(mx_dequant_kernel<FMT, 3, true>, mx_dequant_kernel<FMT, 3, false>);
   }
 }
 
@@ -478,13 +812,49 @@ int norm_launch(const NormParams& p, cudaStream_t s) {
   const int64_t rows = (p.rows + 127) / 128 * 128;
   const int64_t grid = rows / (NT / TR);
   if (grid > kMaxGrid) return B200_ERR_SHAPE;
-  return launch(mx_rms_norm_kernel<FMT, DT, TR, CH>, dim3(unsigned(grid)), NT, p, s);
+  return launch(p.wide ? mx_rms_norm_kernel<FMT, DT, TR, CH, true> : mx_rms_norm_kernel<FMT, DT, TR, CH, false>,
+                dim3(unsigned(grid)), NT, 1, p, s);
 }
 
-// Threads per row: the fewest whose 16-element chunks cover the row and its scale groups.
+template <int FMT, int DT, int NT, int CH>
+int norm_stream(const NormParams& p, int sms, int dev, cudaStream_t s) {
+  auto kern = mx_rms_norm_stream_kernel<FMT, DT, NT, CH>;
+  const size_t smem = size_t(kNormStages) * p.cols * 2 * (p.residual ? 2 : 1);
+  static std::atomic<int> configured[64];
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(reinterpret_cast<const void*>(kern), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kNormSmem) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return B200_ERR_LAUNCH;
+    }
+    configured[dev].store(1, std::memory_order_release);
+  }
+  int per_sm = int((224 * 1024) / (smem + 1536));
+  constexpr int most = 1024 / NT;  // about 64 registers per thread
+  if (per_sm > most) per_sm = most;
+  if (per_sm < 1) per_sm = 1;
+  return launch(kern, dim3(unsigned(sms * per_sm)), NT, 1, p, s, smem);
+}
+
+// Many aligned rows of a 16-bit type stream through shared memory, otherwise a row gets as
+// many threads as its 16-element chunks and scale groups. Streaming wins from 4096 columns
+// on (8192 x 8192 with a residual, MX_FP8: 77-81 us against 95; 8192 x 12288: 128 against
+// 187) and where a power of two of threads would leave many idle (8192 x 2560: 27 against
+// 33); it loses at 2048 x 4096 (14.9 against 13.0). fp32 rows bring twice the bytes per
+// thread and run at the copy rate as they are (8192 x 8192: 133 us, 164 streamed).
 template <int FMT, int DT>
-int norm_t(const NormParams& p, cudaStream_t s) {
+int norm_t(const NormParams& p, int sms, int dev, cudaStream_t s) {
   const int64_t chunks = p.groups * 4 * MxFmt<FMT>::BLOCK / 16;
+  constexpr int es = DT == B200_DT_F32 ? 4 : 2;
+  const int64_t row = p.cols * es * (p.residual ? 2 : 1);
+  const bool idle = chunks > 128 && chunks <= 256 && chunks * 8 < 256 * 7;
+  const bool stream = es == 2 && p.stream && p.rows >= 4 * int64_t(sms) && (idle || chunks > 256) && chunks <= 1024 &&
+                      row * kNormStages <= kNormSmem;
+  if constexpr (es == 2) {
+    if (stream && chunks <= 256) return norm_stream<FMT, DT, 256, 1>(p, sms, dev, s);
+    if (stream && chunks <= 512) return norm_stream<FMT, DT, 512, 1>(p, sms, dev, s);
+    if (stream) return norm_stream<FMT, DT, 512, 2>(p, sms, dev, s);
+  }
   if (chunks <= 32) return norm_launch<FMT, DT, 32, 1>(p, s);
   if (chunks <= 64) return norm_launch<FMT, DT, 64, 1>(p, s);
   if (chunks <= 128) return norm_launch<FMT, DT, 128, 1>(p, s);
@@ -495,11 +865,11 @@ int norm_t(const NormParams& p, cudaStream_t s) {
 }
 
 template <int FMT>
-int norm_f(int dt, const NormParams& p, cudaStream_t s) {
+int norm_f(int dt, const NormParams& p, int sms, int dev, cudaStream_t s) {
   switch (dt) {
-    case B200_DT_F16: return norm_t<FMT, 0>(p, s);
-    case B200_DT_BF16: return norm_t<FMT, 1>(p, s);
-    default: return norm_t<FMT, 3>(p, s);
+    case B200_DT_F16: return norm_t<FMT, 0>(p, sms, dev, s);
+    case B200_DT_BF16: return norm_t<FMT, 1>(p, sms, dev, s);
+    default: return norm_t<FMT, 3>(p, sms, dev, s);
   }
 }
 
@@ -551,27 +921,32 @@ int b200_mx_quantize(const void* x, int32_t x_dtype, int64_t ldx, int32_t transp
   } else if (!find_scale) {
     return B200_OK;
   }
-  int dev = 0, sms = 0;
-  rc = b200::gemm_device(&dev, &sms, nullptr);
+  int sms = 0;
+  rc = b200::gemm_device(nullptr, &sms, nullptr);
   if (rc != B200_OK) return rc;
   const int64_t xrows = transpose ? q->cols : q->rows, xcols = transpose ? q->rows : q->cols;
   const bool wide32 = aligned(x, 32) && (ldx * es) % 32 == 0;
   const bool wide16 = aligned(x, 16) && (ldx * es) % 16 == 0;
+  uint32_t n_partials = 0;
   if (find_scale) {
+    if (q->rows == 0 || q->cols == 0) {  // nothing to look at: 1
+      return launch(mx_unit_scale_kernel, dim3(1), 1, 1, q->tensor_scale, s);
+    }
+    const AmaxParams ap{x, xrows, xcols, ldx, 0, wide32, q->tensor_scale + 4};
     switch (x_dtype) {
-      case B200_DT_F16: rc = amax_t<0>(x, xrows, xcols, ldx, wide32, q->tensor_scale, sms, s); break;
-      case B200_DT_BF16: rc = amax_t<1>(x, xrows, xcols, ldx, wide32, q->tensor_scale, sms, s); break;
-      default: rc = amax_t<3>(x, xrows, xcols, ldx, wide32, q->tensor_scale, sms, s); break;
+      case B200_DT_F16: rc = amax_t<0>(ap, &n_partials, s); break;
+      case B200_DT_BF16: rc = amax_t<1>(ap, &n_partials, s); break;
+      default: rc = amax_t<3>(ap, &n_partials, s); break;
     }
     if (rc != B200_OK) return rc;
-    if (q->rows == 0 || q->cols == 0) return B200_OK;
   }
   QuantParams p{x, q->rows, q->cols, ldx, static_cast<uint8_t*>(q->data), static_cast<uint8_t*>(q->scales),
-                q->tensor_scale, q->ld, mx_groups(q->format, q->cols), transpose ? wide16 : wide32};
+                q->tensor_scale, find_scale ? q->tensor_scale + 4 : nullptr, n_partials, q->ld, mx_groups(q->format, q->cols),
+                transpose ? wide16 : wide32};
   switch (q->format) {
-    case B200_MX_FP8: return quantize_f<MX_FP8>(x_dtype, p, transpose != 0, s);
-    case B200_MX_FP4: return quantize_f<MX_FP4>(x_dtype, p, transpose != 0, s);
-    default: return quantize_f<NV_FP4>(x_dtype, p, transpose != 0, s);
+    case B200_MX_FP8: return quantize_f<MX_FP8>(x_dtype, p, transpose != 0, sms, s);
+    case B200_MX_FP4: return quantize_f<MX_FP4>(x_dtype, p, transpose != 0, sms, s);
+    default: return quantize_f<NV_FP4>(x_dtype, p, transpose != 0, sms, s);
   }
 }
 
@@ -613,9 +988,11 @@ int b200_mx_rms_norm(const B200MxNormArgs* a, const B200MxTensor* q, void* strea
   const int ws = elem_size(a->weight_dtype);
   if (!aligned(a->x, es) || !aligned(a->weight, ws) || !aligned(a->residual, es) || !aligned(a->h, es))
     return B200_ERR_ALIGN;
-  rc = b200::gemm_device(nullptr, nullptr, nullptr);
-  if (rc != B200_OK) return rc;
+  int dev = 0, sms = 0;
   NormParams p{};
+  rc = b200::gemm_device(&dev, &sms, &p.status);
+  if (rc != B200_OK) return rc;
+  p.wait_ns = 1000000000ull;  // 1 s per device wait
   p.x = a->x;
   p.weight = a->weight;
   p.residual = a->residual;
@@ -632,15 +1009,18 @@ int b200_mx_rms_norm(const B200MxNormArgs* a, const B200MxTensor* q, void* strea
   p.tensor_scale = q->tensor_scale;
   p.ld = q->ld;
   p.groups = mx_groups(q->format, q->cols);
-  p.wide = aligned(a->x, 32) && aligned(a->weight, 32) && (a->ldx * es) % 32 == 0 &&
+  p.wide_weight = aligned(a->weight, 32);
+  p.wide = aligned(a->x, 32) && (a->ldx * es) % 32 == 0 &&
            (!a->residual || (aligned(a->residual, 32) && aligned(a->h, 32) && (a->ldr * es) % 32 == 0 &&
                              (a->ldh * es) % 32 == 0));
   p.weight_f32 = a->weight_dtype == B200_DT_F32;
+  p.stream = (q->cols * es) % 16 == 0 && aligned(a->x, 16) && (a->ldx * es) % 16 == 0 &&
+             (!a->residual || (aligned(a->residual, 16) && (a->ldr * es) % 16 == 0));
   cudaStream_t s = static_cast<cudaStream_t>(stream_v);
   switch (q->format) {
-    case B200_MX_FP8: return norm_f<MX_FP8>(a->dtype, p, s);
-    case B200_MX_FP4: return norm_f<MX_FP4>(a->dtype, p, s);
-    default: return norm_f<NV_FP4>(a->dtype, p, s);
+    case B200_MX_FP8: return norm_f<MX_FP8>(a->dtype, p, sms, dev, s);
+    case B200_MX_FP4: return norm_f<MX_FP4>(a->dtype, p, sms, dev, s);
+    default: return norm_f<NV_FP4>(a->dtype, p, sms, dev, s);
   }
 }
 

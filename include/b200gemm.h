@@ -241,8 +241,9 @@ int b200_mx_layout(int32_t format, int64_t rows, int64_t cols, int64_t* row_byte
  * is not finite) gets a NaN scale and makes every sum it enters NaN.
  * find_scale != 0 (B200_NV_FP4): the tensor scale is max|x| / 2688 over the finite
  * elements (at least 2^-126; 1 when all are 0), written to q->tensor_scale, which then
- * points to 16 writable bytes, 16-byte aligned (the other 12 are scratch). Otherwise the
- * scale at q->tensor_scale is used as given: positive and normal. */
+ * points to B200_MX_SCALE_BYTES writable bytes, 16-byte aligned (the others are scratch).
+ * Otherwise the scale at q->tensor_scale is used as given: positive and normal. */
+#define B200_MX_SCALE_BYTES 272
 int b200_mx_quantize(const void* x, int32_t x_dtype, int64_t ldx, int32_t transpose, int32_t find_scale,
                      const B200MxTensor* q, void* stream);
 

@@ -117,7 +117,7 @@ def test_quantize_refusals(b200):
     assert call(0x40002, 3, 256, 0, 0, d) == -3
     assert call(0x40000, 1, 256, 0, 1, d) == -1      # no tensor scale to find in an MX format
     assert call(0x40000, 1, 256, 0, 1, _desc(b200, format=2)) == -1
-    assert call(0x40000, 1, 256, 0, 1, _desc(b200, format=2, tensor_scale=0x30004)) == -3  # 16 bytes are written
+    assert call(0x40000, 1, 256, 0, 1, _desc(b200, format=2, tensor_scale=0x30004)) == -3  # not 16-byte aligned
     assert call(0x40000, 1, 256, 0, 0, _desc(b200, rows=0)) == 0
     if not _gpu():
         assert call(0x40000, 1, 256, 0, 1, nv) == b200.ERR_CUDA

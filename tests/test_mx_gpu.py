@@ -108,6 +108,21 @@ def test_quantize_finds_the_tensor_scale(b200, dtype, transpose):
     _check_quantized(b200, t, np.full(x64.T.shape if transpose else x64.shape, 2.0), ts)
 
 
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_large(b200, fmt, dtype, transpose):
+    """Several segments per row and warp, several clusters behind the found scale; once as one
+    matrix without gaps, once as a slice."""
+    for x in (_input(9, 1300, 8200, dtype), _input(10, 1100, 2600, dtype)[:, 3:2500]):
+        t = b200.quantize_mx(x, fmt, transpose=transpose)
+        x64 = _f64(x)
+        ts = np.float32(np.abs(x64).max()) / np.float32(2688.0) if fmt == "nvfp4" else None
+        if ts is not None:
+            assert float(t.tensor_scale) == float(ts)
+        _check_quantized(b200, t, x64.T if transpose else x64, ts)
+
+
 def test_quantize_zero_matrix(b200):
     for fmt in FMTS:
         t = b200.quantize_mx(torch.zeros(130, 70, device="cuda", dtype=torch.bfloat16), fmt)
@@ -371,6 +386,25 @@ def test_rms_norm(b200, fmt, dtype, rows, cols, residual):
         assert (np.abs(_f64(h) - h64) <= tol).all()
     else:
         assert h is None
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cols,residual", [(2056, True), (4096, False), (4096, True), (7000, True), (12000, False)])
+def test_rms_norm_many_rows(b200, fmt, dtype, cols, residual):
+    """Enough rows for the streaming kernel (with a ragged last band), h in place of the
+    residual; x has a row pitch of its own."""
+    rows = 601
+    x = _input(cols, rows, cols + 8, dtype)[:, :cols]
+    r = _input(cols + 1, rows, cols, dtype) if residual else None
+    w = (1 + 0.2 * torch.randn(cols, generator=torch.Generator().manual_seed(cols))).to(DT[dtype]).cuda()
+    y, h64 = _norm_ref(_f64(x), _f64(w), _f64(r) if residual else None, 1e-6)
+    t, h = b200.rms_norm_mx(x, w, r, fmt=fmt, residual_out=r)
+    _ok(b200)
+    _check_norm(t, y)
+    if residual:
+        assert h is r
+        assert (np.abs(_f64(h) - h64) <= (HALF_STEP[dtype] + 2.0 ** -24) * np.abs(h64)).all()
 
 
 @pytest.mark.parametrize("fmt", FMTS)
