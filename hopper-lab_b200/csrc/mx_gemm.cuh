@@ -471,75 +471,72 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       : "memory");
 }
 
-// 32 consecutive fp32 accumulators of one C row, scaled and rounded, as whole 32-byte
-// sectors (a 32-byte aligned address).
+// One lane's 64 accumulators of a C row, scaled and rounded: 32 words of a 16-bit type (then
+// both halves of a TN = 384 tile fit the registers at once) or 64 of fp32.
 template <int CD>
-__device__ __forceinline__ void store_c32(uint8_t* c, uint64_t index, const uint32_t (&r)[32], float scale) {
-  using E = typename OutElem<CD>::E;
-  typename E::T* d = reinterpret_cast<typename E::T*>(c) + index;
-  if constexpr (CD == DT_F32) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(__uint_as_float(r[8 * j + i]) * scale);
-      st_global_v8(d + 8 * j, w);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        w[i] = E::pack(__uint_as_float(r[16 * j + 2 * i]) * scale, __uint_as_float(r[16 * j + 2 * i + 1]) * scale);
-      st_global_v8(d + 16 * j, w);
-    }
-  }
-}
-
-// The same for a warp's 32 rows x 32 columns at any pitch and column count: 64 bytes of
-// each row go through the warp's shared buffer (16-byte chunk j of row l at chunk
-// j ^ (l / 2 % 4), so neither side has bank conflicts) and leave element by element along
-// the rows. One lane per row storing its own elements touched 32 sectors per store: 777 x
-// 5001 x 2200 took 73 us that way.
-template <int CD>
-__device__ __forceinline__ void store_c32_any(uint8_t* c, uint64_t ldc, uint32_t row0, uint32_t rows, uint32_t col0,
-                                              uint32_t cols, const uint32_t (&r)[32], float scale, uint32_t buf) {
+struct CRow {
   using E = typename OutElem<CD>::E;
   using T = typename E::T;
-  const uint32_t lane = lane_id();
-  constexpr uint32_t W = 64 / sizeof(T);  // columns per pass
+  static constexpr uint32_t PER = 4 / sizeof(T);  // columns per word
+  uint32_t w[64 / PER];
+
+  // from 32 accumulators, columns 32 * half on
+  __device__ __forceinline__ void set(const uint32_t (&r)[32], uint32_t half, float scale) {
 #pragma unroll
-  for (uint32_t x = 0; x < 32; x += W) {
-    uint32_t w[16];
-#pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) {
-      if constexpr (CD == DT_F32) w[i] = __float_as_uint(__uint_as_float(r[x + i]) * scale);
-      else w[i] = E::pack(__uint_as_float(r[x + 2 * i]) * scale, __uint_as_float(r[x + 2 * i + 1]) * scale);
+    for (uint32_t i = 0; i < 32 / PER; ++i) {
+      if constexpr (PER == 1) w[32 * half + i] = __float_as_uint(__uint_as_float(r[i]) * scale);
+      else w[16 * half + i] = E::pack(__uint_as_float(r[2 * i]) * scale, __uint_as_float(r[2 * i + 1]) * scale);
     }
-    __syncwarp();
+  }
+
+  // Columns [32 * half, 32 * half + 32) as whole 32-byte sectors (a 32-byte aligned address).
+  __device__ __forceinline__ void store(uint32_t half, uint8_t* c, uint64_t index) const {
+    T* d = reinterpret_cast<T*>(c) + index;
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j)
-      st_shared_v4(buf + lane * 64u + ((j ^ (lane / 2 & 3u)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-    __syncwarp();
-    const uint32_t i = lane % W;
-#pragma unroll 4
-    for (uint32_t l = lane / W; l < rows; l += 32 / W) {
+    for (uint32_t j = 0; j < 4 / PER; ++j) {
+      uint32_t v[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) v[i] = w[32 / PER * half + 8 * j + i];
+      st_global_v8(d + 8 * PER * j, v);
+    }
+  }
+
+  // The same for a warp's 32 rows at any pitch and column count: 64 bytes of each row go
+  // through the warp's shared buffer (16-byte chunk j of row l at chunk j ^ (l / 2 % 4), so
+  // neither side has bank conflicts) and leave element by element along the rows. One lane
+  // per row storing its own elements touched 32 sectors per store: 777 x 5001 x 2200 took
+  // 73 us that way, 13 this way.
+  __device__ __forceinline__ void store_any(uint32_t half, uint8_t* c, uint64_t ldc, uint32_t row0, uint32_t rows,
+                                            uint32_t col0, uint32_t cols, uint32_t buf) const {
+    const uint32_t lane = lane_id();
+    constexpr uint32_t W = 64 / sizeof(T);  // columns per pass
+#pragma unroll
+    for (uint32_t x = 0; x < 32; x += W) {
+      const uint32_t* v = w + 32 / PER * half + x;  // x is 0 for 16-bit types
+      __syncwarp();
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j)
+        st_shared_v4(buf + lane * 64u + ((j ^ (lane / 2 & 3u)) << 4), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      __syncwarp();
+      const uint32_t i = lane % W, byte = i * uint32_t(sizeof(T));
       if (x + i < cols) {
-        const uint32_t a = buf + l * 64u + (((i * uint32_t(sizeof(T)) / 16) ^ (l / 2 & 3u)) << 4) + i * uint32_t(sizeof(T)) % 16;
-        T v;
-        if constexpr (CD == DT_F32) {
-          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-        } else {
-          uint16_t u;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(a) : "memory");
-          v = *reinterpret_cast<T*>(&u);
+#pragma unroll 4
+        for (uint32_t l = lane / W; l < rows; l += 32 / W) {
+          const uint32_t a = buf + l * 64u + (((byte / 16) ^ (l / 2 & 3u)) << 4) + byte % 16;
+          T e;
+          if constexpr (PER == 1) {
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(e) : "r"(a) : "memory");
+          } else {
+            uint16_t u;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(a) : "memory");
+            e = *reinterpret_cast<T*>(&u);
+          }
+          reinterpret_cast<T*>(c)[uint64_t(row0 + l) * ldc + col0 + x + i] = e;
         }
-        reinterpret_cast<T*>(c)[uint64_t(row0 + l) * ldc + col0 + x + i] = v;
       }
     }
   }
-}
+};
 
 template <int FMT, int CD, int TN>
 __global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
@@ -704,8 +701,8 @@ __global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
   } else if (warp >= 4) {
     // ================================ epilogue ================================
     // Warp 4 + 4e + q drains lanes 32q ... 32q + 31, columns 64e ... 64e + 63 of each slot
-    // and hands the slot back before it converts and stores. A lane owns one C row: its 64
-    // columns are whole 32-byte sectors, stored straight from registers.
+    // and hands the slot back before it stores. A lane owns one C row: its 64 columns are
+    // whole 32-byte sectors, stored straight from registers.
     const uint32_t q = warp & 3u, e = (warp - 4) >> 2;
     float scale = 1.0f;
     if (p.ts_a) scale *= *p.ts_a;
@@ -717,36 +714,50 @@ __global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
       uint32_t bm, bn;
       tile_to_bmn(tile, p.m_tiles, p.n_tiles, p.group_m, bm, bn);
       const uint32_t row0 = (2 * bm + rank) * 128 + 32 * q;
+      // Both halves of a 16-bit TN = 384 tile are drained before either is stored: the next
+      // tile's MMAs wait for the drain, and behind half the stores of a tile it would come
+      // a microsecond late.
+      constexpr uint32_t HELD = CD == DT_F32 ? 1 : NH;
+      CRow<CD> out[HELD];
 #pragma unroll 1
-      for (uint32_t h = 0; h < NH; ++h) {
-        const uint32_t slot = acc_slot(it, h);
-        uint32_t okw = 0;
-        if (lane == 0) okw = mbar_wait(bar_tfull + 8 * slot, acc_use(it) & 1u, p.wait_ns, abort_flag) ? 1u : 0u;
-        okw = __shfl_sync(0xffffffffu, okw, 0);
-        if (!okw) {
-          if (lane == 0) fail(ST_EPI_TMEM_FULL);
-          ok = false;
-          break;
+      for (uint32_t h0 = 0; h0 < NH && ok; h0 += HELD) {
+#pragma unroll
+        for (uint32_t x = 0; x < HELD; ++x) {
+          const uint32_t slot = acc_slot(it, h0 + x);
+          uint32_t okw = 0;
+          if (lane == 0) okw = mbar_wait(bar_tfull + 8 * slot, acc_use(it) & 1u, p.wait_ns, abort_flag) ? 1u : 0u;
+          okw = __shfl_sync(0xffffffffu, okw, 0);
+          if (!okw) {
+            if (lane == 0) fail(ST_EPI_TMEM_FULL);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t t0 = tmem_base + ((32u * q) << 16) + slot * Cfg::MMA_N + 64u * e;
+          uint32_t r[2][32];
+          tmem_ld_x32(t0, r[0]);
+          tmem_ld_x32(t0 + 32, r[1]);
+          tmem_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty0 + 8 * slot);
+          out[x].set(r[0], 0, scale);
+          out[x].set(r[1], 1, scale);
         }
-        tc_fence_after();
-        const uint32_t t0 = tmem_base + ((32u * q) << 16) + slot * Cfg::MMA_N + 64u * e;
-        uint32_t r[2][32];
-        tmem_ld_x32(t0, r[0]);
-        tmem_ld_x32(t0 + 32, r[1]);
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty0 + 8 * slot);
-        const uint32_t col = bn * TN + h * Cfg::MMA_N + 64u * e;
+        if (!ok) break;
         if (row0 < p.M) {
 #pragma unroll
-          for (uint32_t x = 0; x < 2; ++x) {
-            const uint32_t cx = col + 32u * x;
-            if (p.vec && cx + 32 <= p.N) {
-              if (row0 + lane < p.M) store_c32<CD>(p.c, uint64_t(row0 + lane) * p.ldc + cx, r[x], scale);
-            } else if (cx < p.N) {
-              store_c32_any<CD>(p.c, p.ldc, row0, min(32u, p.M - row0), cx, p.N - cx, r[x], scale,
-                                sEpi + (warp - 4) * 2048u);
+          for (uint32_t x = 0; x < HELD; ++x) {
+            const uint32_t col = bn * TN + (h0 + x) * Cfg::MMA_N + 64u * e;
+#pragma unroll
+            for (uint32_t half = 0; half < 2; ++half) {
+              const uint32_t cx = col + 32u * half;
+              if (p.vec && cx + 32 <= p.N) {
+                if (row0 + lane < p.M) out[x].store(half, p.c, uint64_t(row0 + lane) * p.ldc + cx);
+              } else if (cx < p.N) {
+                out[x].store_any(half, p.c, p.ldc, row0, min(32u, p.M - row0), cx, p.N - cx,
+                                 sEpi + (warp - 4) * 2048u);
+              }
             }
           }
         }

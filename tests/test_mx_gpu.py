@@ -500,3 +500,150 @@ def test_linear_training_step(b200, fmt):
         tx = (N / 32 + 6) * 2.0 ** -23 * float(np.abs(vdy[m]) @ np.abs(vwt[k])) + 1e-9 * abs(loss_x(x64[m, k]))
         tw = (M / 32 + 6) * 2.0 ** -23 * float(np.abs(vdyt[n]) @ np.abs(vxt[k])) + 1e-9 * abs(loss_w(w64[n, k]))
         assert abs(float(dx[m, k]) - gx) <= tx and abs(float(dw[n, k]) - gw) <= tw
+
+
+# ------------------------------------------------------------- streams, graphs, big sizes
+def test_gemm_of_a_matrix_with_itself(b200):
+    rng = np.random.default_rng(8)
+    for fmt in FMTS:
+        for M in (20, 200):
+            code, byte = X.random_operand(rng, M, 300, fmt, exact=True)
+            a = _device_operand(b200, code, byte, fmt, 300)
+            v = X.values(code, byte, fmt, 300)
+            np.testing.assert_array_equal(_f64(b200.gemm_mx(a, a, out_dtype="f32")), v @ v.T)
+
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_other_stream_than_the_current_one(b200, raw):
+    """Inputs made on the side stream behind a long queue; nothing but the stream argument
+    orders the calls after them, and what they allocate belongs to that stream."""
+    side = torch.cuda.Stream()
+    handle = side.cuda_stream if raw else side
+    big = torch.randn(4096, 4096, device="cuda")
+    x, w = torch.zeros(150, 512, device="cuda"), torch.ones(512, device="cuda")
+    r = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            big = big @ big * 1e-3
+        x.normal_()
+        r.normal_()
+    q = b200.quantize_mx(x, "nvfp4", stream=handle)
+    y = b200.dequantize_mx(q, out_dtype="f32", stream=handle)
+    n, h = b200.rms_norm_mx(x, w, r, fmt="nvfp4", stream=handle)
+    c = b200.gemm_mx(n, q, out_dtype="f32", stream=handle)
+    side.synchronize()
+    ts = np.float32(float(x.abs().max())) / np.float32(2688.0)
+    _check_quantized(b200, q, _f64(x), ts)
+    ref, h64 = _norm_ref(_f64(x), _f64(w), _f64(r), 1e-6)
+    _check_norm(n, ref)
+    assert (np.abs(_f64(h) - h64) <= 2.0 ** -23 * np.abs(h64)).all()
+    va, vb = _f64(b200.dequantize_mx(n, out_dtype="f32")), _f64(y)
+    tol = (512 / 32 + 6) * 2.0 ** -23 * (np.abs(va) @ np.abs(vb).T)
+    assert (np.abs(_f64(c) - va @ vb.T) <= tol).all()
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_captured_and_replayed(b200, M):
+    """Norm, quantisation with a found scale and products in a graph, replayed on new inputs;
+    a second graph of the same calls interleaved with it; both give the eager results."""
+    N, K = 390, 1000
+    x = torch.randn(M, K, device="cuda").to(torch.bfloat16)
+    r = torch.randn(M, K, device="cuda").to(torch.bfloat16)
+    w = torch.ones(K, device="cuda", dtype=torch.bfloat16)
+    wt = torch.randn(N, K, device="cuda").to(torch.bfloat16)
+
+    def calls():
+        n, h = b200.rms_norm_mx(x, w, r, fmt="nvfp4")
+        q = b200.quantize_mx(wt, "nvfp4")
+        t = b200.quantize_mx(h, "mxfp8", transpose=True)
+        return b200.gemm_mx(n, q), b200.gemm_mx(t, t, out_dtype="f32"), b200.dequantize_mx(q), h
+
+    calls()
+    side = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = calls()
+        graphs.append((g, out))
+    for k in range(3):
+        for t in (x, r, wt):
+            t.copy_(torch.randn_like(t) * (k + 1))
+        for g, out in graphs:
+            for o in out:
+                o.fill_(float("nan"))
+        for g, _ in graphs + graphs:
+            g.replay()
+        want = calls()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+    _ok(b200)
+
+
+def test_two_streams_at_once(b200):
+    """Split-K and pair products, quantisation and norm on two streams without ordering."""
+    rng = np.random.default_rng(11)
+    jobs = []
+    for fmt, M, N, K in (("nvfp4", 3, 1000, 8192), ("mxfp8", 600, 900, 4096), ("mxfp4", 100, 512, 8192)):
+        ca, ba = X.random_operand(rng, M, K, fmt, exact=True)
+        cb, bb = X.random_operand(rng, N, K, fmt, exact=True)
+        ref = X.values(ca, ba, fmt, K) @ X.values(cb, bb, fmt, K).T
+        jobs.append((_device_operand(b200, ca, ba, fmt, K), _device_operand(b200, cb, bb, fmt, K), ref))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for rep in range(20):
+        for i, (a, b, ref) in enumerate(jobs):
+            outs.append((b200.gemm_mx(a, b, out_dtype="f32", stream=streams[(rep + i) % 2]), ref))
+    torch.cuda.synchronize()
+    _ok(b200)
+    for c, ref in outs:
+        np.testing.assert_array_equal(_f64(c), ref)
+
+
+def test_more_elements_than_32_bits(b200):
+    """4.3e9 elements: every offset (x, elements, scales, C) passes 2^32; the last rows and
+    columns are checked."""
+    rows, cols = 70016, 62016
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[:] = torch.randn(cols, device="cuda").to(torch.bfloat16)
+    x[-200:].normal_()
+    t = b200.quantize_mx(x, "mxfp8")
+    some = _f64(x[-200:])
+    code, byte, _ = X.quantize(some, "mxfp8")
+    np.testing.assert_array_equal(X.unsigned_zero(t.data[-200:].cpu().numpy(), "mxfp8"), X.unsigned_zero(code, "mxfp8"))
+    got = X.scale_bytes(t.scales[-1:].cpu().numpy(), 128, cols // 32)  # 70016 rows are 547 whole bands
+    np.testing.assert_array_equal(got, byte[-128:])
+    y = b200.dequantize_mx(t)
+    assert torch.equal(y[-200:].float().cpu(), torch.from_numpy(X.values(code, byte, "mxfp8", cols).astype(np.float32)))
+    del y
+    u = b200.quantize_mx(x, "mxfp8", transpose=True)  # cols x rows
+    tail = _f64(x[:, -40:]).T
+    code_t, byte_t, _ = X.quantize(tail, "mxfp8")
+    np.testing.assert_array_equal(X.unsigned_zero(u.data[-40:].cpu().numpy(), "mxfp8"),
+                                  X.unsigned_zero(code_t, "mxfp8"))
+    del u
+    w = torch.ones(1, device="cuda").expand(20000).contiguous()
+    n, h = b200.rms_norm_mx(x[:, :20000], w, x[:, 40000:60000], fmt="mxfp8")
+    assert torch.equal(h[-200:], x[-200:, :20000] + x[-200:, 40000:60000])
+    ref, _ = _norm_ref(_f64(x[-8:, :20000]), np.ones(20000), _f64(x[-8:, 40000:60000]), 1e-6)
+    v = _f64(b200.dequantize_mx(n)[-8:])
+    assert (np.abs(v - ref) <= 2.0 ** -4 * np.abs(ref) * 1.01 + 2.0 ** -10 * 0.02).all()
+    del n, h
+    b = b200.quantize_mx(x[-300:], "mxfp8")
+    c = b200.gemm_mx(t, b, out_dtype="f32")  # A beyond 2^32 bytes
+    va, vb = X.values(code, byte, "mxfp8", cols), _f64(b200.dequantize_mx(b, out_dtype="f32"))
+    tol = (cols / 32 + 4) * 2.0 ** -23 * (np.abs(va) @ np.abs(vb).T)
+    assert (np.abs(_f64(c[-200:]) - va @ vb.T) <= tol).all()
+    del t, b, c, x
+    a, b = torch.randn(rows, 64, device="cuda"), torch.randn(cols, 64, device="cuda")
+    qa, qb = b200.quantize_mx(a, "mxfp8"), b200.quantize_mx(b, "mxfp8")
+    c = b200.gemm_mx(qa, qb)  # C beyond 2^32 elements
+    va, vb = _f64(b200.dequantize_mx(qa, out_dtype="f32")), _f64(b200.dequantize_mx(qb, out_dtype="f32"))
+    ref = va[-100:] @ vb[-100:].T
+    tol = 6 * 2.0 ** -23 * (np.abs(va[-100:]) @ np.abs(vb[-100:]).T) + 2.0 ** -8 * np.abs(ref)
+    assert (np.abs(_f64(c[-100:, -100:]) - ref) <= tol).all()
+    _ok(b200)
