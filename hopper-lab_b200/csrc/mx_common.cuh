@@ -336,14 +336,13 @@ __device__ __forceinline__ float mx_inverse_scale(uint32_t byte) {
   return byte == 0xFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((254u - byte) << 23);
 }
 
-// NV_FP4 block scale: RN_e4m3(min(amax / 6, 448)). The division is correctly rounded, and
-// a value amax / 6 that is not a rounding border of e4m3 cannot round onto one (6 * border
-// has 7 significant bits, so amax differs from it by at least one unit of its last place,
-// and a sixth of that is more than half a unit of the quotient's), so the byte is the
-// nearest to the exact quotient.
+// NV_FP4 block scale: nearest e4m3 to min(fl(amax * fl(1/6)), 448). The product with the
+// rounded reciprocal is the definition (one multiplication, the same everywhere); it is
+// within 2^-23 of amax / 6, so a scale differs from the exact quotient's only next to a
+// border between two e4m3 values.
 __device__ __forceinline__ uint32_t nv_scale_byte(uint32_t amax) {
   if (amax >= 0x7F800000u) return 0x7Fu;
-  const float s = fminf(__fdiv_rn(__uint_as_float(amax), 6.0f), 448.0f);
+  const float s = fminf(__uint_as_float(amax) * (1.0f / 6.0f), 448.0f);
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(s));
   return r & 0xFFu;
@@ -352,9 +351,11 @@ __device__ __forceinline__ uint32_t nv_scale_byte(uint32_t amax) {
 // u / s for one NV_FP4 block: one Newton residual step on u * (1/s) with fused
 // multiply-adds (Markstein, "Computation of elementary functions on the IBM RISC
 // System/6000 processor", 1990) gives the correctly rounded quotient for the 4-bit
-// significand of s, so ties between e2m1 values fall as the definition says. By the same
-// spacing argument as above no other quotient rounds onto a tie. Nothing overflows: u / s
-// is below 10 unless s = 448, the largest scale, and then it is below u.
+// significand of s. A border t between two e2m1 values has 3 significant bits, so t * s has 7
+// and is an fp32 number: a u that differs from it does so by at least a unit of its last
+// place, which is more than half a unit of the quotient's, and no such quotient rounds onto
+// t. Ties between e2m1 values therefore fall as those of the exact quotient. Nothing
+// overflows: u / s is below 10 unless s = 448, the largest scale, and then it is below u.
 struct NvInverse {
   float s, r;
   __device__ __forceinline__ explicit NvInverse(uint32_t byte) {

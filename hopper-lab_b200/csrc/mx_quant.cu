@@ -22,7 +22,7 @@ namespace {
 using namespace b200;
 
 // ---------------------------------------------------------------------------------
-// per-tensor scale of NV_FP4: amax / (6 * 448)
+// per-tensor scale of NV_FP4: amax * fl(1 / (6 * 448))
 // ---------------------------------------------------------------------------------
 // The first kernel leaves one maximum of finite magnitudes per cluster of CTAs behind the
 // scale, at most kPartials; every warp of the quantiser reduces them again (the maximum does
@@ -125,7 +125,7 @@ __device__ __forceinline__ float tensor_scale_from(const float* partials, uint32
   uint32_t m = lane < n ? __float_as_uint(partials[lane]) : 0u;
   if (lane + 32 < n) m = max(m, __float_as_uint(partials[lane + 32]));
   m = __reduce_max_sync(0xffffffffu, m);
-  return m ? fmaxf(__fdiv_rn(__uint_as_float(m), 2688.0f), 1.17549435e-38f) : 1.0f;
+  return m ? fmaxf(__uint_as_float(m) * (1.0f / 2688.0f), 1.17549435e-38f) : 1.0f;
 }
 
 // ---------------------------------------------------------------------------------
@@ -438,7 +438,7 @@ struct NormParams {
   const void* residual;  // may be null
   void* h;               // x + residual, rounded; null when there is no residual
   int64_t rows, cols, ldx, ldr, ldh;
-  float eps, inv_cols;
+  float eps, n_cols;
   uint8_t* data;
   uint8_t* scales;
   const float* tensor_scale;
@@ -473,6 +473,19 @@ __device__ __forceinline__ void norm_read16(const uint8_t* a, int n, float (&v)[
       }
     }
   }
+}
+
+// Pairwise: an error of the row's sum moves every element of the row against its rounding
+// borders, so the sum is worth a few more bits than one running total of 16 keeps.
+__device__ __forceinline__ float sum_squares(const float (&v)[16]) {
+  float s[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s[i] = v[i] * v[i];
+#pragma unroll
+    for (int j = 4; j < 16; j += 4) s[i] = fmaf(v[i + j], v[i + j], s[i]);
+  }
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 // The last part of both kernels: one 16-element chunk at column c of row `row`, of which n
@@ -566,8 +579,7 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
       if constexpr (WIDE) store16<DT>(h + c, n == 16, n, v[ch]);
       else warp_store16<DT>(h + wc, warp_left, stage[warp], v[ch]);
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) ss = fmaf(v[ch][i], v[ch][i], ss);
+    ss += sum_squares(v[ch]);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -580,7 +592,7 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) ss += mine[i];
   }
-  float rstd = rsqrtf(fmaf(ss, p.inv_cols, p.eps));
+  float rstd = __frsqrt_rn(__fdiv_rn(ss, p.n_cols) + p.eps);
   if constexpr (FMT == NV_FP4)
     if (p.tensor_scale) rstd *= __frcp_rn(*p.tensor_scale);
 #pragma unroll
@@ -679,7 +691,7 @@ __global__ void __launch_bounds__(NT) mx_rms_norm_stream_kernel(const NormParams
 #pragma unroll
     for (int i = 0; i < NT / 32; ++i) ss += red[parity][i];
     parity ^= 1u;  // the other buffer: a fast warp's next sum must not overtake a slow one's read
-    const float rstd = rsqrtf(fmaf(ss, p.inv_cols, p.eps)) * pre;
+    const float rstd = __frsqrt_rn(__fdiv_rn(ss, p.n_cols) + p.eps) * pre;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * NT + threadIdx.x) * 16;
@@ -780,6 +792,7 @@ int amax_t(AmaxParams p, uint32_t* n_partials, cudaStream_t s) {
   if (p.ld == p.cols && p.rows < (int64_t(1) << 62) / p.cols) {
     p.cols *= p.rows;  // no gaps between the rows: one long row
     p.rows = 1;
+    p.wide = aligned(p.x, 32);
   }
   p.segs = (p.cols + 511) / 512;
   // clusters of 8 CTAs, about two segments to a warp and at most kPartials clusters; a
@@ -1003,7 +1016,7 @@ int b200_mx_rms_norm(const B200MxNormArgs* a, const B200MxTensor* q, void* strea
   p.ldr = a->ldr;
   p.ldh = a->ldh;
   p.eps = a->eps;
-  p.inv_cols = 1.0f / float(q->cols);
+  p.n_cols = float(q->cols);
   p.data = static_cast<uint8_t*>(q->data);
   p.scales = static_cast<uint8_t*>(q->scales);
   p.tensor_scale = q->tensor_scale;

@@ -235,11 +235,11 @@ int b200_mx_layout(int32_t format, int64_t rows, int64_t cols, int64_t* row_byte
  *   MX formats: a block's scale is the smallest 2^e, e >= -127, with amax <= max * 2^e
  *     (max 448 or 6), so no element saturates; element = nearest(x / 2^e).
  *   B200_NV_FP4: u = x * fl32(1 / tensor scale), rounded to fp32; block scale =
- *     nearest_e4m3(min(max|u| / 6, 448)); element = nearest_e2m1(u / block scale),
+ *     nearest_e4m3(min(fl32(max|u| * fl32(1/6)), 448)); element = nearest_e2m1(u / block scale),
  *     saturating at 6; all elements are 0 where the scale rounds to 0.
  * Ties go to the even significand. A block that holds a NaN or an infinity (or a u that
  * is not finite) gets a NaN scale and makes every sum it enters NaN.
- * find_scale != 0 (B200_NV_FP4): the tensor scale is max|x| / 2688 over the finite
+ * find_scale != 0 (B200_NV_FP4): the tensor scale is fl32(max|x| * fl32(1/2688)) over the finite
  * elements (at least 2^-126; 1 when all are 0), written to q->tensor_scale, which then
  * points to B200_MX_SCALE_BYTES writable bytes, 16-byte aligned (the others are scratch).
  * Otherwise the scale at q->tensor_scale is used as given: positive and normal. */

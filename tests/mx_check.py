@@ -47,6 +47,11 @@ def mx_exponent(amax, fmt):
     return e
 
 
+def found_scale(amax):
+    """Tensor scale that the quantiser finds for a largest finite magnitude."""
+    return np.float32(amax) * (np.float32(1) / np.float32(2688))
+
+
 def quantize(x, fmt, tensor_scale=None):
     """(element codes, scale bytes), each (rows, n); x is 64-bit and holds the input exactly.
     Element codes carry the sign in their top bit; -0 is not told from 0."""
@@ -62,7 +67,8 @@ def quantize(x, fmt, tensor_scale=None):
     amax = np.abs(vf).max(-1)
     table, sign = (E4M3, 128) if fmt == "mxfp8" else (E2M1, 8)
     if fmt == "nvfp4":
-        byte = nearest(amax / 6.0, E4M3)
+        with np.errstate(over="ignore"):  # the definition's product, held in fp32
+            byte = nearest(np.float64(np.float32(amax) * (np.float32(1) / np.float32(6))), E4M3)
         s = E4M3[byte]
         q = np.where(s[..., None] > 0, vf / np.where(s > 0, s, 1.0)[..., None], 0.0)
         byte = np.where(bad, 0x7F, byte)

@@ -96,14 +96,14 @@ def test_quantize_finds_the_tensor_scale(b200, dtype, transpose):
     t = b200.quantize_mx(x, "nvfp4", transpose=transpose)
     x64 = _f64(x)
     amax = np.abs(x64[np.isfinite(x64)]).max()
-    ts = np.float32(amax) / np.float32(2688.0)
+    ts = X.found_scale(amax)
     assert float(t.tensor_scale) == float(ts)
     _check_quantized(b200, t, x64.T if transpose else x64, ts)
     # again into the same storage, with other data: the scale is found anew
     y = x * 0 + 2.0
     y[5, 7] = y[6, 200] = 2.0
     b200.quantize_mx(y, "nvfp4", transpose=transpose, out=t)
-    ts = np.float32(2.0) / np.float32(2688.0)
+    ts = X.found_scale(2.0)
     assert float(t.tensor_scale) == float(ts)
     _check_quantized(b200, t, np.full(x64.T.shape if transpose else x64.shape, 2.0), ts)
 
@@ -117,10 +117,23 @@ def test_quantize_large(b200, fmt, dtype, transpose):
     for x in (_input(9, 1300, 8200, dtype), _input(10, 1100, 2600, dtype)[:, 3:2500]):
         t = b200.quantize_mx(x, fmt, transpose=transpose)
         x64 = _f64(x)
-        ts = np.float32(np.abs(x64).max()) / np.float32(2688.0) if fmt == "nvfp4" else None
+        ts = X.found_scale(np.abs(x64).max()) if fmt == "nvfp4" else None
         if ts is not None:
             assert float(t.tensor_scale) == float(ts)
         _check_quantized(b200, t, x64.T if transpose else x64, ts)
+
+
+def test_quantize_coarse_values_meet_scale_borders(b200):
+    """Values of few bits with the tensor scale found: block maxima over the largest element
+    are ratios of small integers, so max|u| / 6 falls on and next to e4m3 borders often."""
+    rng = np.random.default_rng(12)
+    for top in (37, 38, 40, 41, 43, 45, 56, 63):
+        x64 = rng.integers(-top, top + 1, size=(301, 1003)) / 8.0
+        x64[7, 9] = top / 8.0
+        for dtype in ("f16", "bf16"):
+            t = b200.quantize_mx(torch.from_numpy(x64).to(DT[dtype]).cuda(), "nvfp4")
+            assert float(t.tensor_scale) == float(X.found_scale(top / 8.0))
+            _check_quantized(b200, t, x64, X.found_scale(top / 8.0))
 
 
 def test_quantize_zero_matrix(b200):
@@ -533,7 +546,7 @@ def test_other_stream_than_the_current_one(b200, raw):
     n, h = b200.rms_norm_mx(x, w, r, fmt="nvfp4", stream=handle)
     c = b200.gemm_mx(n, q, out_dtype="f32", stream=handle)
     side.synchronize()
-    ts = np.float32(float(x.abs().max())) / np.float32(2688.0)
+    ts = X.found_scale(float(x.abs().max()))
     _check_quantized(b200, q, _f64(x), ts)
     ref, h64 = _norm_ref(_f64(x), _f64(w), _f64(r), 1e-6)
     _check_norm(n, ref)
