@@ -106,6 +106,51 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&r)[8]) {
                : "memory");
 }
 
+// W words from any element-aligned address: the whole 16-byte chunks around them, shifted
+// into place (word selects and one funnel shift, the same code for every offset). Elements
+// read one by one touch 16 times as many sectors. A chunk that reaches outside [lo, hi),
+// the memory that the matrix spans, is put together from its elements inside.
+template <int DT, int W>
+__device__ __forceinline__ void load_words_any(const void* p, const void* lo, const void* hi, uint32_t (&r)[W]) {
+  constexpr uint32_t ES = sizeof(typename Elem<DT>::T);
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), base = a & ~uintptr_t(15);
+  const uintptr_t first = reinterpret_cast<uintptr_t>(lo), end = reinterpret_cast<uintptr_t>(hi);
+  const uint32_t o = uint32_t(a & 15);
+  uint32_t w[W + 4];
+#pragma unroll
+  for (int c = 0; c <= W / 4; ++c) {
+    const uintptr_t at = base + 16 * c;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (c < W / 4 || o != 0) {
+      if (at >= first && at + 16 <= end) {
+        v = *reinterpret_cast<const uint4*>(at);
+      } else {
+        uint32_t e[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t i = 0; i < 16 / ES; ++i) {
+          const uintptr_t q = at + ES * i;
+          if (q >= first && q + ES <= end) {
+            if constexpr (ES == 2) e[i / 2] |= uint32_t(*reinterpret_cast<const uint16_t*>(q)) << (16 * (i & 1));
+            else e[i] = *reinterpret_cast<const uint32_t*>(q);
+          }
+        }
+        v = make_uint4(e[0], e[1], e[2], e[3]);
+      }
+    }
+    w[4 * c] = v.x;
+    w[4 * c + 1] = v.y;
+    w[4 * c + 2] = v.z;
+    w[4 * c + 3] = v.w;
+  }
+  uint32_t t[W + 3], u[W + 1];
+#pragma unroll
+  for (int i = 0; i < W + 3; ++i) t[i] = (o & 4) ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < W + 1; ++i) u[i] = (o & 8) ? t[i + 2] : t[i];
+#pragma unroll
+  for (int i = 0; i < W; ++i) r[i] = ES == 2 ? __funnelshift_r(u[i], u[i + 1], (o & 2) * 8) : u[i];
+}
+
 // 16 consecutive elements as they lie in memory (two to a register for 16-bit types).
 template <int DT>
 struct Raw16 {
@@ -138,6 +183,24 @@ struct Raw16 {
         if constexpr (!PACKED) r[i] = e;
         else if (i & 1) r[i / 2] |= e << 16;
         else r[i / 2] = e;
+      }
+    }
+  }
+  // At any element-aligned address inside a matrix that spans [lo, hi): the `n` existing
+  // ones, the rest zero.
+  __device__ __forceinline__ void load_any(const T* p, int n, const T* lo, const T* hi) {
+    constexpr int W = PACKED ? 8 : 16;
+    if (n > 0) {
+      load_words_any<DT, W>(p, lo, hi, r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) r[i] = 0;
+    }
+    if (n > 0 && n < 16) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if constexpr (PACKED) r[i] = 2 * i >= n ? 0 : 2 * i + 1 >= n ? r[i] & 0xFFFFu : r[i];
+        else r[i] = i >= n ? 0 : r[i];
       }
     }
   }
@@ -189,49 +252,22 @@ __device__ __forceinline__ void store16(typename Elem<DT>::T* p, bool wide, int 
   }
 }
 
-// Rows that do not start on 32 bytes: a warp's 512 consecutive elements go element by
-// element, lanes side by side, and change hands in shared memory (256 at a time), so that
-// every lane still owns 16 consecutive ones. A lane loading or storing its own 16 one by
-// one touches 32 sectors per access instead of 2 or 4 (1001 x 5003 to bf16: 34 us that
-// way for the dequantiser). All lanes take part; `p` is the warp's first element, of which
-// `n` exist (n may be negative).
-constexpr int kStageFloats = 272;  // per warp: 256 and one of padding per 16
 template <int DT>
-__device__ __forceinline__ void warp_load16(const typename Elem<DT>::T* p, int64_t n, float* stage, float (&v)[16]) {
-  const uint32_t lane = lane_id();
-#pragma unroll
-  for (uint32_t half = 0; half < 2; ++half) {
-    float t[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      const uint32_t k = 256 * half + 32 * i + lane;
-      t[i] = int64_t(k) < n ? Elem<DT>::load(p[k]) : 0.0f;
-    }
-    __syncwarp();
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      const uint32_t k = 32 * i + lane;
-      stage[k + k / 16] = t[i];
-    }
-    __syncwarp();
-    if (lane / 16 == half) {
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) v[i] = stage[lane % 16 * 17 + i];
-    }
-  }
+__device__ __forceinline__ void load16_any(const typename Elem<DT>::T* p, int n, const typename Elem<DT>::T* lo,
+                                           const typename Elem<DT>::T* hi, float (&v)[16]) {
+  Raw16<DT> w;
+  w.load_any(p, n, lo, hi);
+  w.unpack(v);
 }
-template <int DT>
-__device__ __forceinline__ void warp_load16(const typename Elem<DT>::T* p, int64_t n, float* stage, Raw16<DT>& w) {
-  float v[16];
-  warp_load16<DT>(p, n, stage, v);
-  if constexpr (Raw16<DT>::PACKED) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w.r[i] = Elem<DT>::pack(v[2 * i], v[2 * i + 1]);  // exact: they came from 16 bits
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w.r[i] = __float_as_uint(v[i]);
-  }
-}
+
+// Store 16 fp32 values per lane, rounded, to a row that starts at any element-aligned
+// address: they change hands in shared memory (256 at a time, kStageFloats of it per warp)
+// and leave lanes side by side. A lane storing its own 16 one by one touches 32 sectors per
+// store (1001 x 5003 to bf16: the dequantiser took 34 us that way, 5.3 this way; 7.7 with
+// whole 16-byte chunks shifted together across lanes, whose ragged ends cost more than they
+// save). All lanes take part; `p` is the warp's first element, of which `n` exist (n may be
+// negative).
+constexpr int kStageFloats = 272;  // 256 and one of padding per 16
 template <int DT>
 __device__ __forceinline__ void warp_store16(typename Elem<DT>::T* p, int64_t n, float* stage, const float (&v)[16]) {
   const uint32_t lane = lane_id();

@@ -52,8 +52,7 @@ __global__ void __launch_bounds__(256, 4) mx_amax_kernel(const AmaxParams p) {
   griddep_wait();
   griddep_launch_dependents();
   using T = typename Elem<DT>::T;
-  constexpr int FLY = WIDE ? (sizeof(T) == 2 ? 4 : 2) : 1;
-  __shared__ float stage[WIDE ? 1 : 8][kStageFloats];
+  constexpr int FLY = sizeof(T) == 2 ? (WIDE ? 4 : 2) : (WIDE ? 2 : 1);
   __shared__ uint32_t red[8];
   __shared__ uint32_t part[kAmaxCluster];
   const T* x = static_cast<const T*>(p.x);
@@ -64,12 +63,10 @@ __global__ void __launch_bounds__(256, 4) mx_amax_kernel(const AmaxParams p) {
     const int64_t row = p.rows == 1 ? 0 : t >> 32 ? t / p.segs : uint32_t(t) / uint32_t(p.segs);
     const int64_t c0 = (t - row * p.segs) * 512, left = p.cols - c0;
     const T* src = x + row * p.ld + c0;
-    if constexpr (WIDE) {
-      const int64_t n = left - 16 * int64_t(lane);
-      w.load(src + 16 * lane, n >= 16, n < 16 ? int(n) : 16);
-    } else {
-      warp_load16<DT>(src, left, stage[warp], w);
-    }
+    const int64_t rest = left - 16 * int64_t(lane);
+    const int n = rest < 16 ? int(rest) : 16;
+    if constexpr (WIDE) w.load(src + 16 * lane, n == 16, n);
+    else w.load_any(src + 16 * lane, n, x, x + (p.rows - 1) * p.ld + p.cols);
   };
   uint32_t m = 0;
   const auto fold = [&](const Raw16<DT>& w) {
@@ -162,24 +159,22 @@ __global__ void __launch_bounds__(256) mx_quant_rows_kernel(const QuantParams p)
   griddep_wait();
   griddep_launch_dependents();
   using T = typename Elem<DT>::T;
-  __shared__ float stage[WIDE ? 1 : 8][kStageFloats];
   const uint32_t lane = lane_id(), warp = warp_id();
   const uint32_t warps_per_row = uint32_t((p.groups * 4 * MxFmt<FMT>::BLOCK + 512 * CH - 1) / (512 * CH));
   const int64_t t = int64_t(blockIdx.x) * 8 + warp;
   const int64_t row = t >> 32 ? t / warps_per_row : uint32_t(t) / warps_per_row;
   if (row >= (p.rows + 127) / 128 * 128) return;  // whole warps
   const int64_t c0 = (t - row * warps_per_row) * (512 * CH);
-  const T* src = static_cast<const T*>(p.x) + row * p.ldx + c0;
+  const T* x = static_cast<const T*>(p.x);
+  const T* src = x + row * p.ldx + c0;
   Raw16<DT> w[CH];
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
     const int64_t left = row < p.rows ? p.cols - c0 - 512 * ch : 0;
-    if constexpr (WIDE) {
-      const int64_t n = left - 16 * int64_t(lane);
-      w[ch].load(src + 512 * ch + 16 * lane, n >= 16, n < 16 ? int(n) : 16);
-    } else {
-      warp_load16<DT>(src + 512 * ch, left, stage[warp], w[ch]);
-    }
+    const int64_t rest = left - 16 * int64_t(lane);
+    const int n = rest < 16 ? int(rest) : 16;
+    if constexpr (WIDE) w[ch].load(src + 512 * ch + 16 * lane, n == 16, n);
+    else w[ch].load_any(src + 512 * ch + 16 * lane, n, x, x + (p.rows - 1) * p.ldx + p.cols);
   }
   float r = 1.0f;
   if constexpr (FMT == NV_FP4) r = scale_reciprocal(p);
@@ -270,10 +265,22 @@ __global__ void __launch_bounds__(128) mx_quant_cols_kernel(const QuantParams p)
       }
     }
   } else {
-#pragma unroll 8
-    for (int i = threadIdx.x; i < 128 * 64; i += 128) {
-      const int k = i / 64, c = i % 64;
-      tile[k][Tile::place(c, k / 32)] = k < kleft && c < cleft ? x[(k0 + k) * p.ldx + c0 + c] : E::store(0.0f);
+    constexpr int kPerRow = 64 / kVec;
+    const T* end = x + (p.cols - 1) * p.ldx + p.rows;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < 128 * kPerRow; i += 128) {
+      const int k = i / kPerRow, c = i % kPerRow * kVec;
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (k < kleft && c < cleft) {
+        load_words_any<DT, 4>(x + (k0 + k) * p.ldx + c0 + c, x, end, w);
+        if (c + kVec > cleft) {  // columns behind the last
+          T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+          for (int l = 0; l < kVec; ++l)
+            if (c + l >= cleft) e[l] = E::store(0.0f);
+        }
+      }
+      *reinterpret_cast<uint4*>(&tile[k][Tile::place(c, k / 32)]) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
   __syncthreads();
@@ -379,7 +386,6 @@ __global__ void __launch_bounds__(256) mx_dequant_kernel(const DequantParams p) 
   griddep_wait();
   griddep_launch_dependents();
   using T = typename Elem<DT>::T;
-  __shared__ float stage[WIDE ? 1 : 8][kStageFloats];
   const uint32_t warps_per_row = uint32_t((p.cols + 511) / 512);
   const int64_t t = int64_t(blockIdx.x) * 8 + warp_id();
   const int64_t row = t >> 32 ? t / warps_per_row : uint32_t(t) / warps_per_row;
@@ -425,6 +431,7 @@ __global__ void __launch_bounds__(256) mx_dequant_kernel(const DequantParams p) 
     const int64_t left = mine ? p.cols - c : 0;
     store16<DT>(static_cast<T*>(p.y) + row * p.ldy + c, left >= 16, left < 16 ? int(left) : 16, v);
   } else {
+    __shared__ float stage[8][kStageFloats];
     warp_store16<DT>(static_cast<T*>(p.y) + row * p.ldy + c0, p.cols - c0, stage[warp_id()], v);
   }
 }
@@ -472,6 +479,20 @@ __device__ __forceinline__ void norm_read16(const uint8_t* a, int n, float (&v)[
         v[4 * j + i] = __uint_as_float(u[i]);
       }
     }
+  }
+}
+
+// 16 weights at column c, of which n exist, through L1 (every row reads them).
+template <int DT>
+__device__ __forceinline__ void load_weight(const NormParams& p, int c, int n, float (&w)[16]) {
+  if (p.weight_f32) {
+    const float* g = static_cast<const float*>(p.weight);
+    if (p.wide_weight && n == 16) load16<3, true>(g + c, true, n, w);
+    else load16_any<3>(g + c, n, g, g + p.cols, w);
+  } else {
+    const auto* g = static_cast<const typename Elem<DT>::T*>(p.weight);
+    if (p.wide_weight && n == 16) load16<DT, true>(g + c, true, n, w);
+    else load16_any<DT>(g + c, n, g, g + p.cols, w);
   }
 }
 
@@ -553,31 +574,35 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
   constexpr int NT = TR < 256 ? 256 : TR;
   constexpr int ROWS = NT / TR;       // rows per CTA
   constexpr int WARPS = TR / 32;      // warps per row
-  __shared__ float stage[WIDE ? 1 : NT / 32][kStageFloats];
   const int r_in = threadIdx.x / TR, t = threadIdx.x % TR;
   const uint32_t warp = warp_id(), lane = lane_id();
   const int64_t row = int64_t(blockIdx.x) * ROWS + r_in;
   const bool live = row < p.rows;     // rows behind the last only write zero scales
-  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const T* x0 = static_cast<const T*>(p.x);
+  const T* x = x0 + row * p.ldx;
   float v[CH][16];
   float ss = 0.0f;
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
-    const int c = (ch * TR + t) * 16, wc = c - 16 * int(lane);  // this thread's column, its warp's
-    const int warp_left = live ? int(p.cols) - wc : 0;
-    const int n = min(16, max(0, warp_left - 16 * int(lane)));
+    const int c = (ch * TR + t) * 16;
+    const int n = min(16, max(0, live ? int(p.cols) - c : 0));
     if constexpr (WIDE) load16<DT>(x + c, n == 16, n, v[ch]);
-    else warp_load16<DT>(x + wc, warp_left, stage[warp], v[ch]);
+    else load16_any<DT>(x + c, n, x0, x0 + (p.rows - 1) * p.ldx + p.cols, v[ch]);
     if (p.residual) {
-      const T* res = static_cast<const T*>(p.residual) + row * p.ldr;
+      const T* r0 = static_cast<const T*>(p.residual);
+      const T* res = r0 + row * p.ldr;
       T* h = static_cast<T*>(p.h) + row * p.ldh;
       float r[16];
       if constexpr (WIDE) load16<DT>(res + c, n == 16, n, r);
-      else warp_load16<DT>(res + wc, warp_left, stage[warp], r);
+      else load16_any<DT>(res + c, n, r0, r0 + (p.rows - 1) * p.ldr + p.cols, r);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[ch][i] += r[i];
       if constexpr (WIDE) store16<DT>(h + c, n == 16, n, v[ch]);
-      else warp_store16<DT>(h + wc, warp_left, stage[warp], v[ch]);
+      if constexpr (!WIDE) {
+        __shared__ float stage[NT / 32][kStageFloats];
+        const int wc = c - 16 * int(lane);  // the warp's first column
+        warp_store16<DT>(h + wc, live ? int(p.cols) - wc : 0, stage[warp], v[ch]);
+      }
     }
     ss += sum_squares(v[ch]);
   }
@@ -601,8 +626,7 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
     if (c - 16 * int(lane) >= p.groups * (4 * MxFmt<FMT>::BLOCK)) continue;  // the whole warp is behind the row
     const int n = min(16, max(0, live ? int(p.cols) - c : 0));
     float w[16];
-    if (p.weight_f32) load16<3, true>(static_cast<const float*>(p.weight) + c, p.wide_weight && n == 16, n, w);
-    else load16<DT, true>(static_cast<const T*>(p.weight) + c, p.wide_weight && n == 16, n, w);
+    load_weight<DT>(p, c, n, w);
     norm_store<FMT>(p, row, live, c, n, rstd, w, v[ch]);
   }
 }
@@ -642,6 +666,8 @@ __global__ void __launch_bounds__(NT) mx_rms_norm_stream_kernel(const NormParams
     bulk_load(dst, x + row * p.ldx, row_bytes, bar);
     if (res) bulk_load(dst + row_bytes, res + row * p.ldr, row_bytes, bar);
   };
+  // behind the ring, only there when h is at an odd pitch
+  float* stage = reinterpret_cast<float*>(smem + kNormStages * stage_bytes) + warp * kStageFloats;
   const int64_t first = blockIdx.x, step = gridDim.x;
   if (threadIdx.x == 0)
     for (int s = 0; s < kNormStages; ++s)
@@ -675,7 +701,8 @@ __global__ void __launch_bounds__(NT) mx_rms_norm_stream_kernel(const NormParams
         norm_read16<DT>(sx + row_bytes + c * sizeof(T), n, r);
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[ch][i] += r[i];
-        store16<DT>(h + c, p.wide && n == 16, n, v[ch]);
+        if (p.wide) store16<DT>(h + c, n == 16, n, v[ch]);
+        else warp_store16<DT>(h + c - 16 * int(lane), int(p.cols) - c + 16 * int(lane), stage, v[ch]);
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) ss = fmaf(v[ch][i], v[ch][i], ss);
@@ -698,8 +725,7 @@ __global__ void __launch_bounds__(NT) mx_rms_norm_stream_kernel(const NormParams
       const int n = min(16, max(0, int(p.cols) - c));
       if (c - 16 * int(lane) >= p.groups * (4 * MxFmt<FMT>::BLOCK)) continue;
       float w[16];
-      if (p.weight_f32) load16<3, true>(static_cast<const float*>(p.weight) + c, p.wide_weight && n == 16, n, w);
-      else load16<DT, true>(static_cast<const T*>(p.weight) + c, p.wide_weight && n == 16, n, w);
+      load_weight<DT>(p, c, n, w);
       norm_store<FMT>(p, row, true, c, n, rstd, w, v[ch]);
     }
     if (++s == kNormStages) {
@@ -755,7 +781,7 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 int elem_size(int dt) { return dt == B200_DT_F32 ? 4 : (dt == B200_DT_F16 || dt == B200_DT_BF16) ? 2 : 0; }
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
-constexpr int kNormSmem = 220 * 1024;  // of a streaming CTA's rows
+constexpr int kNormSmem = 224 * 1024;  // most of a streaming CTA's shared memory
 
 template <int FMT, int DT>
 int quantize_t(const QuantParams& p, bool transpose, int sms, cudaStream_t s) {
@@ -764,14 +790,16 @@ int quantize_t(const QuantParams& p, bool transpose, int sms, cudaStream_t s) {
     // bf16: MX_FP8 34.6 -> 33.2 us, NV_FP4 44.4 -> 38.4; fp32 has 64 with one), unless that
     // leaves SMs without their 64 warps.
     const int64_t rows = (p.rows + 127) / 128 * 128, segs = (p.groups * 4 * MxFmt<FMT>::BLOCK + 511) / 512;
-    const bool two = p.wide && DT != B200_DT_F32 && segs > 1 && rows * segs >= int64_t(sms) * 64;
+    const bool two = DT != B200_DT_F32 && segs > 1 && rows * segs >= int64_t(sms) * 64;
     const int64_t grid = (rows * (two ? (segs + 1) / 2 : segs) + 7) / 8;
     if (grid > kMaxGrid) return B200_ERR_SHAPE;
     const dim3 g{unsigned(grid)};
-    if (!p.wide) return launch(mx_quant_rows_kernel<FMT, DT, 1, false>, g, 256, 1, p, s);
     if constexpr (DT != B200_DT_F32)
-      if (two) return launch(mx_quant_rows_kernel<FMT, DT, 2, true>, g, 256, 1, p, s);
-    return launch(mx_quant_rows_kernel<FMT, DT, 1, true>, g, 256, 1, p, s);
+      if (two)
+        return launch(p.wide ? mx_quant_rows_kernel<FMT, DT, 2, true> : mx_quant_rows_kernel<FMT, DT, 2, false>, g, 256,
+                      1, p, s);
+    return launch(p.wide ? mx_quant_rows_kernel<FMT, DT, 1, true> : mx_quant_rows_kernel<FMT, DT, 1, false>, g, 256, 1,
+                  p, s);
   }
   const int64_t grid = ((p.rows + 127) / 128 * 2) * ((p.cols + 127) / 128);
   if (grid > kMaxGrid) return B200_ERR_SHAPE;
@@ -832,7 +860,8 @@ int norm_launch(const NormParams& p, cudaStream_t s) {
 template <int FMT, int DT, int NT, int CH>
 int norm_stream(const NormParams& p, int sms, int dev, cudaStream_t s) {
   auto kern = mx_rms_norm_stream_kernel<FMT, DT, NT, CH>;
-  const size_t smem = size_t(kNormStages) * p.cols * 2 * (p.residual ? 2 : 1);
+  const size_t smem = size_t(kNormStages) * p.cols * 2 * (p.residual ? 2 : 1) +
+                      (p.residual && !p.wide ? NT / 32 * kStageFloats * sizeof(float) : 0);
   static std::atomic<int> configured[64];
   if (!configured[dev].load(std::memory_order_acquire)) {
     if (cudaFuncSetAttribute(reinterpret_cast<const void*>(kern), cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -862,7 +891,7 @@ int norm_t(const NormParams& p, int sms, int dev, cudaStream_t s) {
   const int64_t row = p.cols * es * (p.residual ? 2 : 1);
   const bool idle = chunks > 128 && chunks <= 256 && chunks * 8 < 256 * 7;
   const bool stream = es == 2 && p.stream && p.rows >= 4 * int64_t(sms) && (idle || chunks > 256) && chunks <= 1024 &&
-                      row * kNormStages <= kNormSmem;
+                      row * kNormStages <= kNormSmem - 18 * 1024;
   if constexpr (es == 2) {
     if (stream && chunks <= 256) return norm_stream<FMT, DT, 256, 1>(p, sms, dev, s);
     if (stream && chunks <= 512) return norm_stream<FMT, DT, 512, 1>(p, sms, dev, s);

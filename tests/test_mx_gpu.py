@@ -410,6 +410,11 @@ def test_rms_norm_many_rows(b200, fmt, dtype, cols, residual):
     rows = 601
     x = _input(cols, rows, cols + 8, dtype)[:, :cols]
     r = _input(cols + 1, rows, cols, dtype) if residual else None
+    if cols == 7000:  # h at an odd pitch
+        h1 = torch.full((rows, cols + 3), 4.0, dtype=DT[dtype], device="cuda")
+        b200.rms_norm_mx(x, torch.ones(cols, device="cuda"), r, fmt=fmt, residual_out=h1[:, 1:cols + 1])
+        assert torch.equal(h1[:, 1:cols + 1], x + r)
+        assert bool((h1[:, 0] == 4).all()) and bool((h1[:, cols + 1:] == 4).all())
     w = (1 + 0.2 * torch.randn(cols, generator=torch.Generator().manual_seed(cols))).to(DT[dtype]).cuda()
     y, h64 = _norm_ref(_f64(x), _f64(w), _f64(r) if residual else None, 1e-6)
     t, h = b200.rms_norm_mx(x, w, r, fmt=fmt, residual_out=r)
