@@ -208,7 +208,9 @@ int launch_pair(const Call& k) {
   p.ts_b = k.b->tensor_scale;
   p.c = static_cast<uint8_t*>(k.c);
   p.ldc = uint64_t(k.ldc);
-  p.vec = reinterpret_cast<uintptr_t>(k.c) % 32 == 0 && k.ldc * elem_size(k.cd) % 32 == 0;
+  const uint64_t bits = reinterpret_cast<uintptr_t>(k.c) | (uint64_t(k.ldc) * uint64_t(elem_size(k.cd)));
+  p.align = 32;
+  while (bits % p.align) p.align /= 2;
   p.status = k.status;
   p.wait_ns = kWaitNs;
 

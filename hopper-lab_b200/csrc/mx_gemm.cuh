@@ -428,7 +428,7 @@ struct MxPairParams {
   const float* ts_b;
   uint8_t* c;
   uint64_t ldc;   // elements
-  uint32_t vec;   // C rows are 32-byte aligned
+  uint32_t align;  // of C's rows: 32, 16, 8, 4 or 2 bytes
   uint32_t* status;
   uint64_t wait_ns;
 };
@@ -502,14 +502,17 @@ struct CRow {
   }
 
   // The same for a warp's 32 rows at any pitch and column count: 64 bytes of each row go
-  // through the warp's shared buffer (16-byte chunk j of row l at chunk j ^ (l / 2 % 4), so
-  // neither side has bank conflicts) and leave element by element along the rows. One lane
-  // per row storing its own elements touched 32 sectors per store: 777 x 5001 x 2200 took
-  // 73 us that way, 13 this way.
+  // through the warp's shared buffer (16-byte chunk j of row l at chunk j ^ (l / 2 % 4)) and
+  // leave along the rows, VB bytes per lane: 8, 4, or one 16-bit element, as C is aligned.
+  // One lane per row storing its own elements one by one touched 32 sectors per store (777 x
+  // 5001 x 2200: 73 us, 12.5 this way). 4000 x N x 500 MXFP4 with N = 4000, 4004, 4002, 4001:
+  // 10.9, 13.4, 15.3, 16.0 us; rows at odd addresses leave sectors in parts.
+  template <uint32_t VB>
   __device__ __forceinline__ void store_any(uint32_t half, uint8_t* c, uint64_t ldc, uint32_t row0, uint32_t rows,
                                             uint32_t col0, uint32_t cols, uint32_t buf) const {
     const uint32_t lane = lane_id();
-    constexpr uint32_t W = 64 / sizeof(T);  // columns per pass
+    constexpr uint32_t ES = sizeof(T), W = 64 / ES;  // columns per pass
+    constexpr uint32_t LPR = 64 / VB;                // lanes per row
 #pragma unroll
     for (uint32_t x = 0; x < 32; x += W) {
       const uint32_t* v = w + 32 / PER * half + x;  // x is 0 for 16-bit types
@@ -518,20 +521,31 @@ struct CRow {
       for (uint32_t j = 0; j < 4; ++j)
         st_shared_v4(buf + lane * 64u + ((j ^ (lane / 2 & 3u)) << 4), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
       __syncwarp();
-      const uint32_t i = lane % W, byte = i * uint32_t(sizeof(T));
-      if (x + i < cols) {
-#pragma unroll 4
-        for (uint32_t l = lane / W; l < rows; l += 32 / W) {
-          const uint32_t a = buf + l * 64u + (((byte / 16) ^ (l / 2 & 3u)) << 4) + byte % 16;
-          T e;
-          if constexpr (PER == 1) {
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(e) : "r"(a) : "memory");
-          } else {
-            uint16_t u;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(a) : "memory");
-            e = *reinterpret_cast<T*>(&u);
+      const uint32_t byte = lane % LPR * VB, col = x + byte / ES;
+      T* d = reinterpret_cast<T*>(c) + uint64_t(row0) * ldc + col0 + col;
+      const bool whole = col + VB / ES <= cols;
+#pragma unroll 8
+      for (uint32_t l0 = 0; l0 < 32; l0 += 32 / LPR) {
+        const uint32_t l = l0 + lane / LPR;
+        const uint32_t a = buf + l * 64u + (((byte / 16) ^ (l / 2 & 3u)) << 4) + byte % 16;
+        T* at = d + uint64_t(l) * ldc;
+        if constexpr (VB == 2) {
+          uint16_t u;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(a) : "memory");
+          if (whole && l < rows) *reinterpret_cast<uint16_t*>(at) = u;
+        } else {
+          uint32_t u[VB / 4];
+          if constexpr (VB == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u[0]) : "r"(a) : "memory");
+          else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(u[0]), "=r"(u[VB / 4 - 1]) : "r"(a) : "memory");
+          if (whole && l < rows) {
+            if constexpr (VB == 4) *reinterpret_cast<uint32_t*>(at) = u[0];
+            else *reinterpret_cast<uint2*>(at) = make_uint2(u[0], u[VB / 4 - 1]);
+          } else if (col < cols && l < rows) {  // the last column falls inside
+            const T* e = reinterpret_cast<const T*>(u);
+#pragma unroll
+            for (uint32_t i = 0; i < VB / ES; ++i)
+              if (col + i < cols) at[i] = e[i];
           }
-          reinterpret_cast<T*>(c)[uint64_t(row0 + l) * ldc + col0 + x + i] = e;
         }
       }
     }
@@ -752,11 +766,16 @@ __global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
 #pragma unroll
             for (uint32_t half = 0; half < 2; ++half) {
               const uint32_t cx = col + 32u * half;
-              if (p.vec && cx + 32 <= p.N) {
-                if (row0 + lane < p.M) out[x].store(half, p.c, uint64_t(row0 + lane) * p.ldc + cx);
+              const uint64_t at = uint64_t(row0 + lane) * p.ldc + cx;
+              const uint32_t rows = min(32u, p.M - row0), cols = p.N - cx, buf = sEpi + (warp - 4) * 2048u;
+              if (p.align == 32 && cx + 32 <= p.N) {
+                if (lane < rows) out[x].store(half, p.c, at);
               } else if (cx < p.N) {
-                out[x].store_any(half, p.c, p.ldc, row0, min(32u, p.M - row0), cx, p.N - cx,
-                                 sEpi + (warp - 4) * 2048u);
+                if (p.align >= 8) out[x].template store_any<8>(half, p.c, p.ldc, row0, rows, cx, cols, buf);
+                else if (CD == DT_F32 || p.align == 4)
+                  out[x].template store_any<4>(half, p.c, p.ldc, row0, rows, cx, cols, buf);
+                else if constexpr (CD != DT_F32)
+                  out[x].template store_any<2>(half, p.c, p.ldc, row0, rows, cx, cols, buf);
               }
             }
           }

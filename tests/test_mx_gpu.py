@@ -308,19 +308,22 @@ def test_gemm_real_data(b200, fmt, dtype, M, N, K):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("M", [3, 140, 300])
-def test_gemm_strided_output(b200, fmt, M):
-    """A column slice of a wider matrix at an odd offset: only its columns are written."""
-    rng = np.random.default_rng(M)
-    N, K = 261, 416
+@pytest.mark.parametrize("N,pitch,first", [(261, 268, 3), (262, 272, 2), (260, 264, 4), (248, 264, 8), (250, 272, 16),
+                                           (255, 257, 0)])
+def test_gemm_strided_output(b200, fmt, M, N, pitch, first):
+    """A column slice of a wider matrix, at every alignment of its rows: only its columns are
+    written."""
+    rng = np.random.default_rng(M + N)
+    K = 416
     ca, ba = X.random_operand(rng, M, K, fmt, exact=True)
     cb, bb = X.random_operand(rng, N, K, fmt, exact=True)
     a, b = _device_operand(b200, ca, ba, fmt, K), _device_operand(b200, cb, bb, fmt, K)
-    for dtype in ("f32", "f16"):
-        buf = torch.full((M, N + 7), 5.0, dtype=DT[dtype], device="cuda")
-        b200.gemm_mx(a, b, buf[:, 3:3 + N])
-        ref = torch.from_numpy(X.values(ca, ba, fmt, K) @ X.values(cb, bb, fmt, K).T).float().to(DT[dtype]).cuda()
-        assert torch.equal(buf[:, 3:3 + N], ref)
-        assert bool((buf[:, :3] == 5).all()) and bool((buf[:, 3 + N:] == 5).all())
+    ref = torch.from_numpy(X.values(ca, ba, fmt, K) @ X.values(cb, bb, fmt, K).T).float()
+    for dtype in ("f32", "f16", "bf16"):
+        buf = torch.full((M, pitch), 5.0, dtype=DT[dtype], device="cuda")
+        b200.gemm_mx(a, b, buf[:, first:first + N])
+        assert torch.equal(buf[:, first:first + N], ref.to(DT[dtype]).cuda())
+        assert bool((buf[:, :first] == 5).all()) and bool((buf[:, first + N:] == 5).all())
 
 
 @pytest.mark.parametrize("fmt", FMTS)
