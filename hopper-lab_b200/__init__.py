@@ -394,7 +394,8 @@ def quantize_e4m3(x, q=None, scale=None, stream=None):
 
 # ------------------------------------------------------------------ microscaled operands
 # These calls are short kernels, so their host side is kept short too: one allocation for a
-# microscaled matrix, views of it only when asked for, raw stream handles.
+# microscaled matrix, views of it only when asked for, raw stream handles, names looked up
+# once (_mx_setup).
 
 
 def mx_layout(fmt: str, rows: int, cols: int) -> tuple[int, int]:
@@ -458,9 +459,9 @@ class MxTensor:
         else:
             groups, row_bytes, code = (kp + 127) // 128, kp // 2, 1
         scale_bytes = (rows + 127) // 128 * groups * 512
-        torch = _torch()
-        self = object.__new__(cls)
-        self._own = buf = torch.empty(scale_bytes + _MX_GAP + rows * row_bytes, dtype=torch.uint8, device=device)
+        self = _new_object(cls)
+        self._own = buf = (_empty or _mx_setup())(scale_bytes + _MX_GAP + rows * row_bytes, dtype=_uint8,
+                                                  device=device)
         self._off = scale_bytes
         ptr = buf.data_ptr()
         self._data = self._scales = self._ts = None
@@ -514,41 +515,49 @@ class MxTensor:
 
 
 _MX_TORCH = {}  # torch dtype -> code and the names of output types -> (torch dtype, code)
+_empty = _empty_strided = _uint8 = _get_device = _raw_stream = None
+_new_object = object.__new__
 
 
-def _mx_types():
-    if not _MX_TORCH:
-        torch = _torch()
-        for dt, code, names in ((torch.float16, DT_F16, ("f16", "fp16", "float16")),
-                                (torch.bfloat16, DT_BF16, ("bf16", "bfloat16")),
-                                (torch.float32, DT_F32, ("f32", "fp32", "float32"))):
-            _MX_TORCH[dt] = code
-            for name in names + (code,):
-                _MX_TORCH[name] = (dt, code)
-    return _MX_TORCH
+def _mx_setup():
+    global _empty, _empty_strided, _uint8, _get_device, _raw_stream
+    torch = _torch()
+    for dt, code, names in ((torch.float16, DT_F16, ("f16", "fp16", "float16")),
+                            (torch.bfloat16, DT_BF16, ("bf16", "bfloat16")),
+                            (torch.float32, DT_F32, ("f32", "fp32", "float32"))):
+        for name in names + (code,):
+            _MX_TORCH[name] = (dt, code)
+        _MX_TORCH[dt] = code
+    _uint8, _empty_strided = torch.uint8, torch.empty_strided
+    _get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    lib()
+    _empty = torch.empty  # last: the others are there once it is
+    return _empty
 
 
 def _mx_input(name, t):
     """dtype code and row stride of a 2-D fp tensor with unit column stride."""
-    dt = (_MX_TORCH or _mx_types()).get(t.dtype)
+    if _empty is None:
+        _mx_setup()
+    dt = _MX_TORCH.get(t.dtype)
     if dt is None:
         raise TypeError(f"{name} must be float16, bfloat16 or float32, not {t.dtype}")
-    shape = t.shape
-    if len(shape) != 2:
+    stride = t.stride()
+    if len(stride) != 2:
         raise ValueError(f"{name} must be a 2-D row-major tensor with unit column stride")
-    ld, unit = t.stride()
-    if unit != 1 and shape[1] > 1 and shape[0] > 0:
+    rows, cols = t.shape
+    if stride[1] != 1 and cols > 1 and rows > 0:
         raise ValueError(f"{name} must be a 2-D row-major tensor with unit column stride")
-    return dt, ld if shape[0] > 1 else max(shape[1], 1)
+    return dt, stride[0] if rows > 1 else cols or 1
 
 
 def _mx_output(name, rows, cols, device):
     """A new matrix of the named output type, its code and row stride."""
-    kind = (_MX_TORCH or _mx_types()).get(name)
+    kind = _MX_TORCH.get(name)
     if type(kind) is not tuple:
         raise ValueError(f"output type {name!r} is not f16, bf16 or f32")
-    ld = max(cols, 1)
-    return _torch().empty_strided((rows, cols), (ld, 1), dtype=kind[0], device=device), kind[1], ld
+    ld = cols or 1
+    return _empty_strided((rows, cols), (ld, 1), dtype=kind[0], device=device), kind[1], ld
 
 
 def _mx_out(out, rows, cols, fmt, device, tensor_scale):
@@ -595,10 +604,12 @@ class _On:
 def _here(device, stream):
     """Handle of the current stream for a call on the current device and stream, else None:
     the call then makes them current (_On) and starts over."""
-    if stream is None and device.index is not None:
-        cuda = _torch()._C
-        if cuda._cuda_getDevice() == device.index:
-            return cuda._cuda_getCurrentRawStream(device.index)
+    index = device.index
+    if stream is None and index is not None:
+        if _empty is None:
+            _mx_setup()
+        if _get_device() == index:
+            return _raw_stream(index)
     return None
 
 
@@ -621,7 +632,7 @@ def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=
     find = fmt == "nvfp4" and tensor_scale is None
     if find:
         t._scratch()
-    rc = (_LIB or lib()).b200_mx_quantize(x.data_ptr(), dt, ldx, transpose, find, t._ref, here)
+    rc = _LIB.b200_mx_quantize(x.data_ptr(), dt, ldx, transpose, find, t._ref, here)
     if rc != OK:
         raise B200Error(rc, "b200_mx_quantize")
     return t
@@ -640,7 +651,7 @@ def dequantize_mx(t: MxTensor, out=None, *, out_dtype="bf16", stream=None):
         if tuple(out.shape) != t.shape or out.device != device:
             raise ValueError(f"out is {tuple(out.shape)} on {out.device}, needed {t.shape} on {device}")
         dt, ldy = _mx_input("out", out)
-    rc = (_LIB or lib()).b200_mx_dequantize(t._ref, out.data_ptr(), dt, ldy, here)
+    rc = _LIB.b200_mx_dequantize(t._ref, out.data_ptr(), dt, ldy, here)
     if rc != OK:
         raise B200Error(rc, "b200_mx_dequantize")
     return out
@@ -664,7 +675,7 @@ def gemm_mx(a: MxTensor, b: MxTensor, c=None, *, out_dtype="bf16", stream=None):
         if tuple(c.shape) != (a.rows, b.rows) or c.device != device:
             raise ValueError(f"C is {tuple(c.shape)} on {c.device}, needed {(a.rows, b.rows)} on {device}")
         dt, ldc = _mx_input("C", c)
-    rc = (_LIB or lib()).b200_mx_gemm(a._ref, b._ref, c.data_ptr(), dt, ldc, here)
+    rc = _LIB.b200_mx_gemm(a._ref, b._ref, c.data_ptr(), dt, ldc, here)
     if rc != OK:
         raise B200Error(rc, "b200_mx_gemm")
     return c
@@ -710,7 +721,7 @@ def rms_norm_mx(x, weight, residual=None, *, eps: float = 1e-6, fmt: str = "mxfp
         args = MxNormArgs(dt, wt, x.data_ptr(), weight.data_ptr(), residual.data_ptr(), residual_out.data_ptr(),
                           ldx, ldr, ldh, eps, 0)
     t = _mx_out(out, rows, cols, fmt, device, tensor_scale)
-    rc = (_LIB or lib()).b200_mx_rms_norm(C.byref(args), t._ref, here)
+    rc = _LIB.b200_mx_rms_norm(C.byref(args), t._ref, here)
     if rc != OK:
         raise B200Error(rc, "b200_mx_rms_norm")
     return t, residual_out
