@@ -237,33 +237,20 @@ __global__ void __launch_bounds__(128) mx_quant_cols_kernel(const QuantParams p)
   const T* x = static_cast<const T*>(p.x);
   const int64_t kleft = p.cols - k0, cleft = p.rows - c0;
   if (p.wide) {
+    // asynchronous copies: the whole tile is in flight and takes no registers (8192 x 8192
+    // fp32 72 us through registers, eight at a time); what lies outside x reads as zero
     constexpr int kPerRow = 64 / kVec;
-    constexpr int kLoads = 128 * kPerRow / 128;  // per thread: 8 or 16, eight in flight
 #pragma unroll
-    for (int b = 0; b < kLoads; b += 8) {
-      uint4 w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = (b + j) * 128 + threadIdx.x, k = i / kPerRow, c = i % kPerRow * kVec;
-        w[j] = make_uint4(0, 0, 0, 0);
-        if (k < kleft && c < cleft) {
-          const T* src = x + (k0 + k) * p.ldx + c0 + c;
-          if (c + kVec <= cleft) {
-            w[j] = __ldcs(reinterpret_cast<const uint4*>(src));
-          } else {
-            alignas(16) T e[kVec];
-#pragma unroll
-            for (int l = 0; l < kVec; ++l) e[l] = c + l < cleft ? src[l] : E::store(0.0f);
-            w[j] = *reinterpret_cast<const uint4*>(e);
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = (b + j) * 128 + threadIdx.x, k = i / kPerRow, c = i % kPerRow * kVec;
-        *reinterpret_cast<uint4*>(&tile[k][Tile::place(c, k / 32)]) = w[j];
-      }
+    for (int j = 0; j < kPerRow; ++j) {
+      const int i = j * 128 + threadIdx.x, k = i / kPerRow, c = i % kPerRow * kVec;
+      const int64_t left = k < kleft ? cleft - c : 0;
+      const uint32_t bytes = left >= kVec ? 16u : left > 0 ? uint32_t(left) * sizeof(T) : 0u;
+      const T* src = bytes ? x + (k0 + k) * p.ldx + c0 + c : x;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(&tile[k][Tile::place(c, k / 32)])),
+                   "l"(src), "r"(bytes)
+                   : "memory");
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     constexpr int kPerRow = 64 / kVec;
     const T* end = x + (p.cols - 1) * p.ldx + p.rows;
