@@ -12,6 +12,7 @@
 
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #include "b200gemm.h"
 #include "gemm_internal.h"
@@ -432,7 +433,7 @@ struct NormParams {
   const void* residual;  // may be null
   void* h;               // x + residual, rounded; null when there is no residual
   int64_t rows, cols, ldx, ldr, ldh;
-  float eps, n_cols;
+  float eps, inv_cols;
   uint8_t* data;
   uint8_t* scales;
   const float* tensor_scale;
@@ -469,18 +470,19 @@ __device__ __forceinline__ void norm_read16(const uint8_t* a, int n, float (&v)[
   }
 }
 
-// 16 weights at column c, of which n exist, through L1 (every row reads them).
-template <int DT>
+// 16 weights at column c, of which n exist, through L1 (every row reads them). ANY: rows at
+// odd addresses, whose ends are ragged too.
+template <int DT, bool ANY>
 __device__ __forceinline__ void load_weight(const NormParams& p, int c, int n, float (&w)[16]) {
-  if (p.weight_f32) {
-    const float* g = static_cast<const float*>(p.weight);
-    if (p.wide_weight && n == 16) load16<3, true>(g + c, true, n, w);
-    else load16_any<3>(g + c, n, g, g + p.cols, w);
-  } else {
-    const auto* g = static_cast<const typename Elem<DT>::T*>(p.weight);
-    if (p.wide_weight && n == 16) load16<DT, true>(g + c, true, n, w);
-    else load16_any<DT>(g + c, n, g, g + p.cols, w);
-  }
+  const auto load = [&](auto dt, const auto* g) {
+    constexpr int D = decltype(dt)::value;
+    if constexpr (ANY) {
+      if (!p.wide_weight || n < 16) return load16_any<D>(g + c, n, g, g + p.cols, w);
+    }
+    load16<D, true>(g + c, p.wide_weight && n == 16, n, w);
+  };
+  if (p.weight_f32) load(std::integral_constant<int, 3>{}, static_cast<const float*>(p.weight));
+  else load(std::integral_constant<int, DT>{}, static_cast<const typename Elem<DT>::T*>(p.weight));
 }
 
 // Pairwise: an error of the row's sum moves every element of the row against its rounding
@@ -494,6 +496,22 @@ __device__ __forceinline__ float sum_squares(const float (&v)[16]) {
     for (int j = 4; j < 16; j += 4) s[i] = fmaf(v[i + j], v[i + j], s[i]);
   }
   return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// n values (a power of two) added pairwise.
+template <int N>
+__device__ __forceinline__ float sum_of(const float* v) {
+  if constexpr (N == 1) return v[0];
+  else return sum_of<N / 2>(v) + sum_of<N / 2>(v + N / 2);
+}
+
+// 1 / sqrt(m) by one Newton step from rsqrtf: every thread of a row computes it, so it has to
+// be short (a correctly rounded division and root cost 10 % of an 8192-wide row). 0 and
+// infinity keep their rsqrtf.
+__device__ __forceinline__ float reciprocal_root(float m) {
+  const float r = rsqrtf(m);
+  const float e = fmaf(-(m * r), r, 1.0f);
+  return e == e ? fmaf(0.5f * r, e, r) : r;
 }
 
 // The last part of both kernels: one 16-element chunk at column c of row `row`, of which n
@@ -599,12 +617,9 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
     __shared__ float red[NT / 32];
     if (lane == 0) red[warp] = ss;
     __syncthreads();
-    const float* mine = red + r_in * WARPS;
-    ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) ss += mine[i];
+    ss = sum_of<WARPS>(red + r_in * WARPS);
   }
-  float rstd = __frsqrt_rn(__fdiv_rn(ss, p.n_cols) + p.eps);
+  float rstd = reciprocal_root(fmaf(ss, p.inv_cols, p.eps));
   if constexpr (FMT == NV_FP4)
     if (p.tensor_scale) rstd *= __frcp_rn(*p.tensor_scale);
 #pragma unroll
@@ -613,7 +628,7 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
     if (c - 16 * int(lane) >= p.groups * (4 * MxFmt<FMT>::BLOCK)) continue;  // the whole warp is behind the row
     const int n = min(16, max(0, live ? int(p.cols) - c : 0));
     float w[16];
-    load_weight<DT>(p, c, n, w);
+    load_weight<DT, !WIDE>(p, c, n, w);
     norm_store<FMT>(p, row, live, c, n, rstd, w, v[ch]);
   }
 }
@@ -629,7 +644,7 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
 constexpr int kNormStages = 3;
 
 template <int FMT, int DT, int NT, int CH>
-__global__ void __launch_bounds__(NT) mx_rms_norm_stream_kernel(const NormParams p) {
+__global__ void __launch_bounds__(NT, CH == 1 ? 1024 / NT : 1) mx_rms_norm_stream_kernel(const NormParams p) {
   using T = typename Elem<DT>::T;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[2][NT / 32];
@@ -701,18 +716,16 @@ __global__ void __launch_bounds__(NT) mx_rms_norm_stream_kernel(const NormParams
     if (!ok) break;
     // every thread has read the stage: refill it
     if (threadIdx.x == 0 && row + kNormStages * step < p.rows) load_row(row + kNormStages * step, s);
-    ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) ss += red[parity][i];
+    ss = sum_of<NT / 32>(red[parity]);
     parity ^= 1u;  // the other buffer: a fast warp's next sum must not overtake a slow one's read
-    const float rstd = __frsqrt_rn(__fdiv_rn(ss, p.n_cols) + p.eps) * pre;
+    const float rstd = reciprocal_root(fmaf(ss, p.inv_cols, p.eps)) * pre;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * NT + threadIdx.x) * 16;
       const int n = min(16, max(0, int(p.cols) - c));
       if (c - 16 * int(lane) >= p.groups * (4 * MxFmt<FMT>::BLOCK)) continue;
       float w[16];
-      load_weight<DT>(p, c, n, w);
+      load_weight<DT, false>(p, c, n, w);
       norm_store<FMT>(p, row, true, c, n, rstd, w, v[ch]);
     }
     if (++s == kNormStages) {
@@ -858,10 +871,19 @@ int norm_stream(const NormParams& p, int sms, int dev, cudaStream_t s) {
     }
     configured[dev].store(1, std::memory_order_release);
   }
-  int per_sm = int((224 * 1024) / (smem + 1536));
-  constexpr int most = 1024 / NT;  // about 64 registers per thread
-  if (per_sm > most) per_sm = most;
-  if (per_sm < 1) per_sm = 1;
+  // as many CTAs as the device holds at once: one more would run its rows after the others
+  static std::atomic<uint64_t> known[64];  // the last answer: shared memory and CTAs per SM
+  uint64_t last = known[dev].load(std::memory_order_relaxed);
+  if (last >> 8 != smem) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, NT, smem) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      return B200_ERR_LAUNCH;
+    }
+    last = uint64_t(smem) << 8 | uint64_t(n);
+    known[dev].store(last, std::memory_order_relaxed);
+  }
+  const int per_sm = int(last & 0xFF);
   return launch(kern, dim3(unsigned(sms * per_sm)), NT, 1, p, s, smem);
 }
 
@@ -1032,7 +1054,7 @@ int b200_mx_rms_norm(const B200MxNormArgs* a, const B200MxTensor* q, void* strea
   p.ldr = a->ldr;
   p.ldh = a->ldh;
   p.eps = a->eps;
-  p.n_cols = float(q->cols);
+  p.inv_cols = 1.0f / float(q->cols);
   p.data = static_cast<uint8_t*>(q->data);
   p.scales = static_cast<uint8_t*>(q->scales);
   p.tensor_scale = q->tensor_scale;
