@@ -685,9 +685,10 @@ def rms_norm_mx(x, weight, residual=None, *, eps: float = 1e-6, fmt: str = "mxfp
                 out: MxTensor | None = None, residual_out=None, stream=None):
     """RMS norm with the residual's addition, to a microscaled matrix: h = x + residual,
     out = quantised(h / sqrt(mean(h^2) + eps) * weight). Returns (out, h), h rounded to x's
-    type, or (out, None) without a residual. ``residual_out`` may be ``residual`` or ``x``.
-    ``weight`` has x's type or is float32; ``tensor_scale`` ("nvfp4") is used as given, None
-    stands for 1, which suits normalised rows (block maxima from 0.006 to 2688)."""
+    type, or (out, None) without a residual. ``residual_out`` may be ``residual`` or ``x``,
+    and overlaps neither otherwise. ``weight`` has x's type or is float32; ``tensor_scale``
+    ("nvfp4") is used as given, None stands for 1, which suits normalised rows (block maxima
+    from 0.006 to 2688)."""
     dt, ldx = _mx_input("x", x)
     device = x.device
     shape = x.shape

@@ -514,6 +514,40 @@ __device__ __forceinline__ float reciprocal_root(float m) {
   return e == e ? fmaf(0.5f * r, e, r) : r;
 }
 
+// A row whose factor is far from 1 (or NaN) takes a detour, so that what fp32 can hold at the
+// ends does not limit what lies between:
+//   * its squares may have left fp32: the sum overflowed, or it and eps are so small that
+//     squares round away. h is then multiplied by a power of two (2^-80 brings the largest
+//     fp32 to 2^48, 2^100 the smallest to 2^-49), summed again (`join` adds the warps' sums)
+//     and normalised as that row with eps times its square, which is the same y;
+//   * h * w below could leave fp32 though y does not (h = 2^60, w = 2^80): h is multiplied by
+//     the factor first. Without this only |y| from 2^120 on overflows.
+// NaN rows stay as they are, rows with an infinity come back with the same sum.
+__device__ __forceinline__ bool far_factor(float rstd) { return !(rstd > 0x1p-8f && rstd < 0x1p10f); }
+template <int CH, typename Join>
+__device__ __forceinline__ float rescale_row(float (&v)[CH][16], float ss, float rstd, float inv_cols, float eps,
+                                             Join&& join) {
+  if (ss > 0x1p120f || (ss < 0x1p-90f && eps < 0x1p-90f)) {
+    const float f = ss > 1.0f ? 0x1p-80f : 0x1p100f;
+    ss = 0.0f;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[ch][i] *= f;
+      ss += sum_squares(v[ch]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    rstd = reciprocal_root(fmaf(join(ss), inv_cols, eps * f * f));
+  }
+  if (!(rstd > 0.0f && rstd < __int_as_float(0x7F800000))) return rstd;
+#pragma unroll
+  for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[ch][i] *= rstd;
+  return 1.0f;
+}
+
 // The last part of both kernels: one 16-element chunk at column c of row `row`, of which n
 // elements exist, from h in fp32 to elements and scales. Elements behind the last column and
 // rows behind the last are zero even where the row's norm is NaN. Whole warps, 512 columns.
@@ -613,13 +647,24 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  __shared__ float red[NT / 32];
   if constexpr (WARPS > 1) {
-    __shared__ float red[NT / 32];
     if (lane == 0) red[warp] = ss;
     __syncthreads();
     ss = sum_of<WARPS>(red + r_in * WARPS);
   }
   float rstd = reciprocal_root(fmaf(ss, p.inv_cols, p.eps));
+  if (far_factor(rstd))  // all threads of the row see the same sum
+    rstd = rescale_row(v, ss, rstd, p.inv_cols, p.eps, [&](float sum) {
+      if constexpr (WARPS > 1) {
+        const auto row_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + r_in), "n"(TR) : "memory"); };
+        row_sync();
+        if (lane == 0) red[warp] = sum;
+        row_sync();
+        sum = sum_of<WARPS>(red + r_in * WARPS);
+      }
+      return sum;
+    });
   if constexpr (FMT == NV_FP4)
     if (p.tensor_scale) rstd *= __frcp_rn(*p.tensor_scale);
 #pragma unroll
@@ -706,8 +751,7 @@ __global__ void __launch_bounds__(NT, CH == 1 ? 1024 / NT : 1) mx_rms_norm_strea
         if (p.wide) store16<DT>(h + c, n == 16, n, v[ch]);
         else warp_store16<DT>(h + c - 16 * int(lane), int(p.cols) - c + 16 * int(lane), stage, v[ch]);
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) ss = fmaf(v[ch][i], v[ch][i], ss);
+      ss += sum_squares(v[ch]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
@@ -717,8 +761,16 @@ __global__ void __launch_bounds__(NT, CH == 1 ? 1024 / NT : 1) mx_rms_norm_strea
     // every thread has read the stage: refill it
     if (threadIdx.x == 0 && row + kNormStages * step < p.rows) load_row(row + kNormStages * step, s);
     ss = sum_of<NT / 32>(red[parity]);
+    float rstd = reciprocal_root(fmaf(ss, p.inv_cols, p.eps));
+    if (far_factor(rstd))  // all threads see the same sum
+      rstd = rescale_row(v, ss, rstd, p.inv_cols, p.eps, [&](float sum) {
+        __syncthreads();
+        if (lane == 0) red[parity][warp] = sum;
+        __syncthreads();
+        return sum_of<NT / 32>(red[parity]);
+      });
+    rstd *= pre;
     parity ^= 1u;  // the other buffer: a fast warp's next sum must not overtake a slow one's read
-    const float rstd = reciprocal_root(fmaf(ss, p.inv_cols, p.eps)) * pre;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
       const int c = (ch * NT + threadIdx.x) * 16;

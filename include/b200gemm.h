@@ -261,7 +261,8 @@ int b200_mx_gemm(const B200MxTensor* a, const B200MxTensor* b, void* c, int32_t 
 /* RMS norm to a microscaled matrix: for each row, h = x + residual (x alone without a
  * residual), y = h / sqrt(mean(h^2) + eps) * weight in fp32, q = quantised y (the tensor
  * scale of a B200_NV_FP4 q is used as given). With a residual, h is also stored, rounded
- * to dtype; h may be the same memory as x or residual. cols <= B200_MX_NORM_MAX_COLS. */
+ * to dtype; h may be x or residual itself (same address and pitch) and overlaps neither
+ * otherwise. cols <= B200_MX_NORM_MAX_COLS. */
 #define B200_MX_NORM_MAX_COLS 32768
 typedef struct B200MxNormArgs {
   int32_t dtype;        /* of x, residual and h: B200_DT_F16 | B200_DT_BF16 | B200_DT_F32 */

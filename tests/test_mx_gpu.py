@@ -457,6 +457,23 @@ def test_rms_norm_zero_and_nan_rows(b200):
         assert not bool(torch.isnan(y[[0, 1, 3]]).any())
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("rows,cols", [(3, 300), (3, 900), (40, 2000), (601, 4096), (601, 4200)])
+@pytest.mark.parametrize("ex,ew", [(60, 80), (-50, -85), (110, 0), (-120, 0)])
+def test_rms_norm_far_magnitudes(b200, fmt, rows, cols, ex, ew):
+    """h * w, or the squares, leave fp32 (or most of its precision) where the normalised value
+    does not."""
+    if fmt == "nvfp4" and ew:  # with the tensor scale that such values need
+        ex, ew = (40, 82) if ex > 0 else (-30, -86)
+    x = _input(cols, rows, cols, "f32") * 2.0 ** ex
+    x = x.to(torch.bfloat16)
+    w = (1 + 0.2 * torch.randn(cols, generator=torch.Generator().manual_seed(cols))).cuda() * 2.0 ** ew
+    ts = torch.tensor([2.0 ** ew], device="cuda") if fmt == "nvfp4" else None
+    t, _ = b200.rms_norm_mx(x, w, eps=0.0, fmt=fmt, tensor_scale=ts)
+    y, _ = _norm_ref(_f64(x), _f64(w), None, 0.0)
+    _check_norm(t, y, None if ts is None else 2.0 ** ew)
+
+
 # ------------------------------------------------------------------- the run of them all
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("M", [1, 20, 260])
