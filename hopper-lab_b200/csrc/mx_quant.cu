@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
 
 // mx_rms_norm_stream_kernel: many rows. The kernel above keeps as many bytes in flight as
 // its threads hold in registers, 32 or 64 each, and stops loading while a row is reduced and
-// stored (8192 x 8192 bf16: 112 us with a residual, 83 without; the bytes alone: 73 and 31).
+// stored (8192 x 8192 bf16 with a residual: 95 us, streamed 76; the bytes alone: 73).
 // Here a CTA takes rows r, r + grid, ... and one thread copies whole rows of x and residual
 // into a ring in shared memory with cp.async.bulk, kNormStages rows ahead, so the loads of
 // the next rows run under everything else. NT threads, CH chunks each. Rows start on 16
@@ -941,10 +941,10 @@ int norm_stream(const NormParams& p, int sms, int dev, cudaStream_t s) {
 
 // Many aligned rows of a 16-bit type stream through shared memory, otherwise a row gets as
 // many threads as its 16-element chunks and scale groups. Streaming wins from 4096 columns
-// on (8192 x 8192 with a residual, MX_FP8: 77-81 us against 95; 8192 x 12288: 128 against
-// 187) and where a power of two of threads would leave many idle (8192 x 2560: 27 against
-// 33); it loses at 2048 x 4096 (14.9 against 13.0). fp32 rows bring twice the bytes per
-// thread and run at the copy rate as they are (8192 x 8192: 133 us, 164 streamed).
+// on (8192 x 8192 with a residual, MX_FP8: 76 us against 95; 8192 x 12288: 138 against 187)
+// and where a power of two of threads would leave many idle (8192 x 2560: 28.9 against 33);
+// it loses at 2048 x 4096 (14.9 against 12.9). fp32 rows bring twice the bytes per thread
+// and run at the copy rate as they are (8192 x 8192: 134 us, 164 streamed).
 template <int FMT, int DT>
 int norm_t(const NormParams& p, int sms, int dev, cudaStream_t s) {
   const int64_t chunks = p.groups * 4 * MxFmt<FMT>::BLOCK / 16;
