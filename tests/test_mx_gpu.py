@@ -284,6 +284,22 @@ def test_gemm_exact_on_integers(b200, fmt, M, N, K):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 1056), (3700, 4000, 160), (8192, 8100, 96), (5000, 5001, 96)])
+def test_gemm_exact_over_several_waves(b200, fmt, M, N, K):
+    """Tiles in several waves, the last one ragged and its last columns partly or wholly behind
+    the matrix; outputs of 16 and 32 bits."""
+    rng = np.random.default_rng(M + N + K)
+    ca, ba = X.random_operand(rng, M, K, fmt, exact=True)
+    cb, bb = X.random_operand(rng, N, K, fmt, exact=True)
+    a, b = _device_operand(b200, ca, ba, fmt, K), _device_operand(b200, cb, bb, fmt, K)
+    ref = torch.from_numpy(X.values(ca, ba, fmt, K)).cuda() @ torch.from_numpy(X.values(cb, bb, fmt, K)).cuda().T
+    for dtype in ("f32", "bf16"):
+        c = b200.gemm_mx(a, b, out_dtype=dtype)
+        _ok(b200)
+        assert torch.equal(c, ref.float().to(DT[dtype]))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
 @pytest.mark.parametrize("M,N,K", [(1, 512, 4096), (24, 1000, 1024), (150, 333, 700), (384, 768, 1536)])
 def test_gemm_real_data(b200, fmt, dtype, M, N, K):
