@@ -1,0 +1,47 @@
+"""Order of cluster operations in the kernels' sources, checked on the CPU.
+
+- ``barrier.cluster.*.aligned`` has to be executed by a whole, converged warp. Code behind a
+  branch on the thread or lane is not converged by itself, so every function that holds such
+  an instruction converges the warp first.
+"""
+import re
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parents[1] / "hopper-lab_b200" / "csrc"
+
+
+def code(path):
+    """A source file without its comments."""
+    return re.sub(r"//[^\n]*|/\*.*?\*/", "", path.read_text(), flags=re.S)
+
+
+def body(text, start):
+    """The braced block that follows position `start`."""
+    i = text.index("{", start)
+    depth = 0
+    for j in range(i, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[j], 0)
+        if depth == 0:
+            return text[i:j + 1]
+    raise AssertionError("unbalanced braces")
+
+
+def sources():
+    return sorted([*CSRC.glob("*.cu"), *CSRC.glob("*.cuh")])
+
+
+def test_warps_converge_before_aligned_cluster_barriers():
+    found = 0
+    for path in sources():
+        text = code(path)
+        for m in re.finditer(r"\bvoid (\w+)\([^)]*\) ", text):
+            block = body(text, m.end() - 1) if text[m.end()] == "{" else ""
+            at = [b.start() for b in re.finditer(r"barrier\.cluster\.\w+[\w.]*\.aligned", block)]
+            if at:
+                found += 1
+                assert "__syncwarp()" in block[:at[0]], f"{path.name}: {m.group(1)}"
+        # nowhere outside a small function of its own
+        assert len(re.findall(r"barrier\.cluster\.\w+[\w.]*\.aligned", text)) == sum(
+            len(re.findall(r"barrier\.cluster\.\w+[\w.]*\.aligned", body(text, m.end() - 1)))
+            for m in re.finditer(r"__forceinline__ void \w+\([^)]*\) (?=\{)", text))
+    assert found
