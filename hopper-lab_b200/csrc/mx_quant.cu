@@ -50,6 +50,7 @@ struct AmaxParams {
 // of fp32) in flight.
 template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256, 4) mx_amax_kernel(const AmaxParams p) {
+  cluster_arrive_started();
   griddep_wait();
   griddep_launch_dependents();
   using T = typename Elem<DT>::T;
@@ -100,6 +101,7 @@ __global__ void __launch_bounds__(256, 4) mx_amax_kernel(const AmaxParams p) {
   m = __reduce_max_sync(0xffffffffu, m);
   if (lane == 0) red[warp] = m;
   __syncthreads();
+  cluster_wait();  // the first CTA of the cluster has started: its shared memory is there
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) m = max(m, red[i]);

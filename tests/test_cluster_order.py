@@ -45,3 +45,21 @@ def test_warps_converge_before_aligned_cluster_barriers():
             len(re.findall(r"barrier\.cluster\.\w+[\w.]*\.aligned", body(text, m.end() - 1)))
             for m in re.finditer(r"__forceinline__ void \w+\([^)]*\) (?=\{)", text))
     assert found
+
+
+REMOTE = r"\b(?:mapa_shared|st_shared_cluster\w*|ld_shared_cluster\w*|mbar_arrive_cluster\w*)\s*\("
+STARTED = r"\b(?:cluster_sync|cluster_wait)\s*\(\s*\)"
+
+
+def test_cluster_has_started_before_remote_shared_memory():
+    found = 0
+    for path in sources():
+        text = code(path)
+        for m in re.finditer(r"__global__ ", text):
+            name = re.search(r"(\w+)\s*\(\s*const", text[m.end():]).group(1)
+            block = body(text, m.end())
+            remote = re.search(REMOTE, block)
+            if remote:
+                found += 1
+                assert re.search(STARTED, block[:remote.start()]), f"{path.name}: {name}"
+    assert found >= 3

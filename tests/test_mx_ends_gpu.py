@@ -1,0 +1,47 @@
+"""GPU tests of the microscaled operators at the ends of what they take, against plain 64-bit
+forms (mx_check.py).
+
+Tolerances
+- a found tensor scale is one fp32 product, so it is compared for equality.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import mx_check as X
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    yield
+    torch.cuda.synchronize()
+
+
+def _ok(b200):
+    rc, bits = b200.status()
+    assert rc == 0, hex(bits)
+
+
+@pytest.mark.parametrize("n", [4096, 8 * 8192 - 512, 8 * 8192, 8 * 8192 + 512, 9 * 65536 + 8192, 600 * 8192 + 32])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_found_scale_sees_every_part(b200, dtype, n):
+    """The largest magnitude in turn in each part of the matrix, so that each CTA of the clusters
+    that look for it holds it once, those of a last cluster that is partly without work too."""
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    x = torch.full((1, n), 0.25, dtype=dt, device="cuda")
+    places = sorted({*np.linspace(0, n - 1, 40).astype(int).tolist(), *range(0, n, max(1, n // 24))})
+    found = []
+    for k, at in enumerate(places):
+        x[0, at] = -(2 + k)
+        found.append((b200.quantize_mx(x, "nvfp4").tensor_scale, 2 + k))
+        x[0, at] = 0.25
+    torch.cuda.synchronize()
+    _ok(b200)
+    for ts, top in found:
+        assert float(ts) == float(X.found_scale(top))
