@@ -106,30 +106,35 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&r)[8]) {
                : "memory");
 }
 
-// W words from any element-aligned address: the whole 16-byte chunks around them, shifted
-// into place (word selects and one funnel shift, the same code for every offset). Elements
-// read one by one touch 16 times as many sectors. A chunk that reaches outside [lo, hi),
-// the memory that the matrix spans, is put together from its elements inside.
+// W words of a row of `len` elements that starts at any element-aligned address, from element
+// c on: the whole 16-byte chunks around them, shifted into place (word selects and one funnel
+// shift, the same code for every offset). Elements read one by one touch 16 times as many
+// sectors. A chunk that reaches outside the row is put together from its elements inside, so
+// nothing beside the row is read (a strided matrix's gaps may hold what another stream writes)
+// and what lies behind its end is zero. Host code too, for the test of its addresses.
 template <int DT, int W>
-__device__ __forceinline__ void load_words_any(const void* p, const void* lo, const void* hi, uint32_t (&r)[W]) {
-  constexpr uint32_t ES = sizeof(typename Elem<DT>::T);
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), base = a & ~uintptr_t(15);
-  const uintptr_t first = reinterpret_cast<uintptr_t>(lo), end = reinterpret_cast<uintptr_t>(hi);
-  const uint32_t o = uint32_t(a & 15);
+__host__ __device__ __forceinline__ void load_words_any(const typename Elem<DT>::T* row, int64_t len, int64_t c0,
+                                                        uint32_t (&r)[W]) {
+  constexpr int ES = sizeof(typename Elem<DT>::T);
+  const uintptr_t a = reinterpret_cast<uintptr_t>(row + c0);
+  const int o = int(a & 15);
+  // bytes of the row ahead of c0 and from it on, as far as they matter here
+  const int lead = int(c0 < 16 ? c0 : 16) * ES, rest = int(len - c0 < 64 ? len - c0 : 64) * ES;
+  const char* base = reinterpret_cast<const char*>(a - o);
   uint32_t w[W + 4];
 #pragma unroll
   for (int c = 0; c <= W / 4; ++c) {
-    const uintptr_t at = base + 16 * c;
+    const int at = 16 * c - o;  // the chunk's place relative to c0
     uint4 v = make_uint4(0, 0, 0, 0);
     if (c < W / 4 || o != 0) {
-      if (at >= first && at + 16 <= end) {
-        v = *reinterpret_cast<const uint4*>(at);
+      if (at >= -lead && at + 16 <= rest) {
+        v = *reinterpret_cast<const uint4*>(base + 16 * c);
       } else {
         uint32_t e[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (uint32_t i = 0; i < 16 / ES; ++i) {
-          const uintptr_t q = at + ES * i;
-          if (q >= first && q + ES <= end) {
+        for (int i = 0; i < 16 / ES; ++i) {
+          const char* q = base + 16 * c + ES * i;
+          if (at + ES * i >= -lead && at + ES * (i + 1) <= rest) {
             if constexpr (ES == 2) e[i / 2] |= uint32_t(*reinterpret_cast<const uint16_t*>(q)) << (16 * (i & 1));
             else e[i] = *reinterpret_cast<const uint32_t*>(q);
           }
@@ -148,7 +153,8 @@ __device__ __forceinline__ void load_words_any(const void* p, const void* lo, co
 #pragma unroll
   for (int i = 0; i < W + 1; ++i) u[i] = (o & 8) ? t[i + 2] : t[i];
 #pragma unroll
-  for (int i = 0; i < W; ++i) r[i] = ES == 2 ? __funnelshift_r(u[i], u[i + 1], (o & 2) * 8) : u[i];
+  for (int i = 0; i < W; ++i)
+    r[i] = ES == 2 ? uint32_t((uint64_t(u[i + 1]) << 32 | u[i]) >> ((o & 2) * 8)) : u[i];
 }
 
 // 16 consecutive elements as they lie in memory (two to a register for 16-bit types).
@@ -186,22 +192,15 @@ struct Raw16 {
       }
     }
   }
-  // At any element-aligned address inside a matrix that spans [lo, hi): the `n` existing
-  // ones, the rest zero.
-  __device__ __forceinline__ void load_any(const T* p, int n, const T* lo, const T* hi) {
+  // Elements c to c + 15 of a row of `len` at any element-aligned address: the existing ones,
+  // the rest zero.
+  __host__ __device__ __forceinline__ void load_any(const T* row, int64_t len, int64_t c) {
     constexpr int W = PACKED ? 8 : 16;
-    if (n > 0) {
-      load_words_any<DT, W>(p, lo, hi, r);
+    if (c < len) {
+      load_words_any<DT, W>(row, len, c, r);
     } else {
 #pragma unroll
       for (int i = 0; i < W; ++i) r[i] = 0;
-    }
-    if (n > 0 && n < 16) {
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        if constexpr (PACKED) r[i] = 2 * i >= n ? 0 : 2 * i + 1 >= n ? r[i] & 0xFFFFu : r[i];
-        else r[i] = i >= n ? 0 : r[i];
-      }
     }
   }
   __device__ __forceinline__ void unpack(float (&v)[16]) const {
@@ -253,10 +252,9 @@ __device__ __forceinline__ void store16(typename Elem<DT>::T* p, bool wide, int 
 }
 
 template <int DT>
-__device__ __forceinline__ void load16_any(const typename Elem<DT>::T* p, int n, const typename Elem<DT>::T* lo,
-                                           const typename Elem<DT>::T* hi, float (&v)[16]) {
+__device__ __forceinline__ void load16_any(const typename Elem<DT>::T* row, int64_t len, int64_t c, float (&v)[16]) {
   Raw16<DT> w;
-  w.load_any(p, n, lo, hi);
+  w.load_any(row, len, c);
   w.unpack(v);
 }
 

@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(256, 4) mx_amax_kernel(const AmaxParams p) {
     const int64_t rest = left - 16 * int64_t(lane);
     const int n = rest < 16 ? int(rest) : 16;
     if constexpr (WIDE) w.load(src + 16 * lane, n == 16, n);
-    else w.load_any(src + 16 * lane, n, x, x + (p.rows - 1) * p.ld + p.cols);
+    else w.load_any(x + row * p.ld, p.cols, c0 + 16 * int64_t(lane));
   };
   uint32_t m = 0;
   const auto fold = [&](const Raw16<DT>& w) {
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(256) mx_quant_rows_kernel(const QuantParams p)
     const int64_t rest = left - 16 * int64_t(lane);
     const int n = rest < 16 ? int(rest) : 16;
     if constexpr (WIDE) w[ch].load(src + 512 * ch + 16 * lane, n == 16, n);
-    else w[ch].load_any(src + 512 * ch + 16 * lane, n, x, x + (p.rows - 1) * p.ldx + p.cols);
+    else w[ch].load_any(x + row * p.ldx, row < p.rows ? p.cols : 0, c0 + 512 * ch + 16 * int64_t(lane));
   }
   float r = 1.0f;
   if constexpr (FMT == NV_FP4) r = scale_reciprocal(p);
@@ -256,20 +256,11 @@ __global__ void __launch_bounds__(128) mx_quant_cols_kernel(const QuantParams p)
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     constexpr int kPerRow = 64 / kVec;
-    const T* end = x + (p.cols - 1) * p.ldx + p.rows;
 #pragma unroll 4
     for (int i = threadIdx.x; i < 128 * kPerRow; i += 128) {
       const int k = i / kPerRow, c = i % kPerRow * kVec;
       uint32_t w[4] = {0, 0, 0, 0};
-      if (k < kleft && c < cleft) {
-        load_words_any<DT, 4>(x + (k0 + k) * p.ldx + c0 + c, x, end, w);
-        if (c + kVec > cleft) {  // columns behind the last
-          T* e = reinterpret_cast<T*>(w);
-#pragma unroll
-          for (int l = 0; l < kVec; ++l)
-            if (c + l >= cleft) e[l] = E::store(0.0f);
-        }
-      }
+      if (k < kleft && c < cleft) load_words_any<DT, 4>(x + (k0 + k) * p.ldx, p.rows, c0 + c, w);
       *reinterpret_cast<uint4*>(&tile[k][Tile::place(c, k / 32)]) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
@@ -479,7 +470,7 @@ __device__ __forceinline__ void load_weight(const NormParams& p, int c, int n, f
   const auto load = [&](auto dt, const auto* g) {
     constexpr int D = decltype(dt)::value;
     if constexpr (ANY) {
-      if (!p.wide_weight || n < 16) return load16_any<D>(g + c, n, g, g + p.cols, w);
+      if (!p.wide_weight || n < 16) return load16_any<D>(g, p.cols, c, w);
     }
     load16<D, true>(g + c, p.wide_weight && n == 16, n, w);
   };
@@ -619,8 +610,8 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
   const uint32_t warp = warp_id(), lane = lane_id();
   const int64_t row = int64_t(blockIdx.x) * ROWS + r_in;
   const bool live = row < p.rows;     // rows behind the last only write zero scales
-  const T* x0 = static_cast<const T*>(p.x);
-  const T* x = x0 + row * p.ldx;
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  const int64_t len = live ? p.cols : 0;
   float v[CH][16];
   float ss = 0.0f;
 #pragma unroll
@@ -628,14 +619,13 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
     const int c = (ch * TR + t) * 16;
     const int n = min(16, max(0, live ? int(p.cols) - c : 0));
     if constexpr (WIDE) load16<DT>(x + c, n == 16, n, v[ch]);
-    else load16_any<DT>(x + c, n, x0, x0 + (p.rows - 1) * p.ldx + p.cols, v[ch]);
+    else load16_any<DT>(x, len, c, v[ch]);
     if (p.residual) {
-      const T* r0 = static_cast<const T*>(p.residual);
-      const T* res = r0 + row * p.ldr;
+      const T* res = static_cast<const T*>(p.residual) + row * p.ldr;
       T* h = static_cast<T*>(p.h) + row * p.ldh;
       float r[16];
       if constexpr (WIDE) load16<DT>(res + c, n == 16, n, r);
-      else load16_any<DT>(res + c, n, r0, r0 + (p.rows - 1) * p.ldr + p.cols, r);
+      else load16_any<DT>(res, len, c, r);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[ch][i] += r[i];
       if constexpr (WIDE) store16<DT>(h + c, n == 16, n, v[ch]);

@@ -45,3 +45,33 @@ def test_found_scale_sees_every_part(b200, dtype, n):
     _ok(b200)
     for ts, top in found:
         assert float(ts) == float(X.found_scale(top))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols,pitch,first", [(1, 1, 9, 3), (5, 7, 9, 1), (70, 33, 47, 5), (131, 517, 523, 3),
+                                                   (200, 1023, 1025, 1)])
+def test_column_slices_are_as_their_copies(b200, dtype, rows, cols, pitch, first):
+    """What lies between the rows of a slice (NaN here) has no part in any result, and a whole
+    matrix gives the same bytes as its slice."""
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    g = torch.Generator().manual_seed(rows + cols)
+    slices = []
+    for _ in range(2):
+        buf = torch.full((rows, pitch), float("nan"), dtype=dt, device="cuda")
+        buf[:, first:first + cols] = torch.randn(rows, cols, generator=g).to(dt).cuda()
+        slices.append(buf[:, first:first + cols])
+    x, r = slices
+    w = torch.full((cols + 5,), float("nan"), dtype=dt, device="cuda")
+    w[5:] = (1 + 0.1 * torch.randn(cols, generator=g)).to(dt).cuda()
+    w = w[5:]
+    for fmt in ("mxfp8", "mxfp4", "nvfp4"):
+        for transpose in (False, True):
+            a = b200.quantize_mx(x, fmt, transpose=transpose)
+            b = b200.quantize_mx(x.contiguous(), fmt, transpose=transpose)
+            assert torch.equal(a.data, b.data) and torch.equal(a.scales, b.scales)
+            if fmt == "nvfp4":
+                assert float(a.tensor_scale) == float(b.tensor_scale) == float(X.found_scale(float(x.abs().max())))
+        a, h = b200.rms_norm_mx(x, w, r, fmt=fmt)
+        b, k = b200.rms_norm_mx(x.contiguous(), w.clone(), r.contiguous(), fmt=fmt)
+        assert torch.equal(a.data, b.data) and torch.equal(a.scales, b.scales) and torch.equal(h, k)
+    _ok(b200)
