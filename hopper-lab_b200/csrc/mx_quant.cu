@@ -597,7 +597,8 @@ __device__ __forceinline__ void norm_store(const NormParams& p, int64_t row, boo
 
 // mx_rms_norm_kernel: TR threads per row, CH chunks of 16 elements per thread. A thread has
 // read its chunk of x and residual before it writes that chunk of h, and no other thread
-// reads it, so h may be x or residual itself.
+// reads it (rows at odd addresses: the row is read before h is written), so h may be x or
+// residual itself.
 template <int FMT, int DT, int TR, int CH, bool WIDE>
 __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const NormParams p) {
   griddep_wait();
@@ -622,20 +623,27 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
     else load16_any<DT>(x, len, c, v[ch]);
     if (p.residual) {
       const T* res = static_cast<const T*>(p.residual) + row * p.ldr;
-      T* h = static_cast<T*>(p.h) + row * p.ldh;
       float r[16];
       if constexpr (WIDE) load16<DT>(res + c, n == 16, n, r);
       else load16_any<DT>(res, len, c, r);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[ch][i] += r[i];
-      if constexpr (WIDE) store16<DT>(h + c, n == 16, n, v[ch]);
-      if constexpr (!WIDE) {
-        __shared__ float stage[NT / 32][kStageFloats];
-        const int wc = c - 16 * int(lane);  // the warp's first column
+      if constexpr (WIDE) store16<DT>(static_cast<T*>(p.h) + row * p.ldh + c, n == 16, n, v[ch]);
+    }
+    ss += sum_squares(v[ch]);
+  }
+  if constexpr (!WIDE) {
+    if (p.residual) {
+      // a thread's whole chunks reach into its neighbours' elements: in place, h waits for them
+      if (p.h == p.x || p.h == p.residual) __syncthreads();
+      T* h = static_cast<T*>(p.h) + row * p.ldh;
+      __shared__ float stage[NT / 32][kStageFloats];
+#pragma unroll
+      for (int ch = 0; ch < CH; ++ch) {
+        const int wc = (ch * TR + t) * 16 - 16 * int(lane);  // the warp's first column
         warp_store16<DT>(h + wc, live ? int(p.cols) - wc : 0, stage[warp], v[ch]);
       }
     }
-    ss += sum_squares(v[ch]);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);

@@ -75,3 +75,23 @@ def test_column_slices_are_as_their_copies(b200, dtype, rows, cols, pitch, first
         b, k = b200.rms_norm_mx(x.contiguous(), w.clone(), r.contiguous(), fmt=fmt)
         assert torch.equal(a.data, b.data) and torch.equal(a.scales, b.scales) and torch.equal(h, k)
     _ok(b200)
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 597), (70, 5743), (20, 20001)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_norm_in_place_at_odd_pitches(b200, dtype, rows, cols):
+    """h written over x or over the residual, at pitches where a thread reads whole chunks around
+    its elements: the same bytes as into a matrix of its own."""
+    dt = {"bf16": torch.bfloat16, "f32": torch.float32}[dtype]
+    g = torch.Generator().manual_seed(cols)
+    x, r = (torch.randn(rows, cols + 2, generator=g).to(dt).cuda()[:, 1:cols + 1] for _ in range(2))
+    w = (1 + 0.1 * torch.randn(cols, generator=g)).to(dt).cuda()
+    want, h = b200.rms_norm_mx(x, w, r)
+    assert torch.equal(h, x + r)
+    for rep in range(5):
+        for over_x in (True, False):
+            bx, br = (torch.empty(rows, cols + 2, dtype=dt, device="cuda") for _ in range(2))
+            a, b = bx[:, 1:cols + 1].copy_(x), br[:, 1:cols + 1].copy_(r)
+            t, k = b200.rms_norm_mx(a, w, b, residual_out=a if over_x else b)
+            assert torch.equal(k, h) and torch.equal(t.data, want.data) and torch.equal(t.scales, want.scales)
+    _ok(b200)
