@@ -193,6 +193,32 @@ struct MxRowsCfg {
   }
 };
 
+// ts_a * ts_b as two factors that a sum is multiplied by one after the other. The product of
+// two tensor scales (positive and normal) may leave fp32 where C does not: A near 1e-30 and B
+// near 1e-8 have scales of 4e-34 and 4e-12, and two large ones overflow, which would make a
+// sum of zero NaN. Inside fp32's normal numbers it is one factor (the other is 1). Sums are
+// multiples of 2^-20 below 2^54, so the first product is normal wherever C is not 0, and
+// infinite only where C is. A negative or NaN scale comes through too.
+struct SumScale {
+  float first, second = 1.0f;
+  __device__ __forceinline__ SumScale(const float* ts_a, const float* ts_b) {
+    const float a = ts_a ? *ts_a : 1.0f, b = ts_b ? *ts_b : 1.0f;
+    first = a * b;
+    if (fabsf(first) < 0x1p-126f && a != 0.0f && b != 0.0f) {  // neither is above 2^23
+      first = (a * 0x1p64f) * (b * 0x1p64f);
+      second = 0x1p-128f;
+    } else if (fabsf(first) > 0x1.fffffep127f) {  // neither is below 1
+      first = (a * 0x1p-63f) * (b * 0x1p-64f);
+      first = fminf(fmaxf(first, -0x1.fffffep127f), 0x1.fffffep127f);
+      second = 0x1p127f;
+    }
+  }
+  template <int FMT>
+  __device__ __forceinline__ float apply(float sum) const {
+    return FMT == NV_FP4 ? sum * first * second : sum;  // the other formats have no tensor scale
+  }
+};
+
 template <int CD>
 struct OutElem;
 template <>
@@ -379,9 +405,7 @@ __global__ void __launch_bounds__(256, 1)
   }
   if (p.splits > 1) cluster_sync();
   if (!*abort_flag) {
-    float scale = 1.0f;
-    if (p.ts_p) scale *= *p.ts_p;
-    if (p.ts_q) scale *= *p.ts_q;
+    const SumScale scale(p.ts_p, p.ts_q);
     const uint32_t rows = min(uint32_t(NT), p.nq - q0);
     const uint32_t col = p0 + 4 * lane;
     const uint32_t ncol = col < p.np ? min(4u, p.np - col) : 0u;
@@ -401,10 +425,10 @@ __global__ void __launch_bounds__(256, 1)
           v.w += w.w;
         }
       }
-      v.x *= scale;
-      v.y *= scale;
-      v.z *= scale;
-      v.w *= scale;
+      v.x = scale.apply<FMT>(v.x);
+      v.y = scale.apply<FMT>(v.y);
+      v.z = scale.apply<FMT>(v.z);
+      v.w = scale.apply<FMT>(v.w);
       store_c4<CD>(p.c, uint64_t(q0 + r) * p.ldc + col, v, ncol, p.vec);
     }
   }
@@ -481,11 +505,20 @@ struct CRow {
   uint32_t w[64 / PER];
 
   // from 32 accumulators, columns 32 * half on
-  __device__ __forceinline__ void set(const uint32_t (&r)[32], uint32_t half, float scale) {
+  template <int FMT>
+  __device__ __forceinline__ void set(uint32_t (&r)[32], uint32_t half, const SumScale& scale) {
+    if constexpr (FMT == NV_FP4) {  // the other formats have no tensor scale
+#pragma unroll
+      for (uint32_t i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale.first);
+      if (scale.second != 1.0f) {  // rare: a branch, not a multiplication each
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * scale.second);
+      }
+    }
 #pragma unroll
     for (uint32_t i = 0; i < 32 / PER; ++i) {
-      if constexpr (PER == 1) w[32 * half + i] = __float_as_uint(__uint_as_float(r[i]) * scale);
-      else w[16 * half + i] = E::pack(__uint_as_float(r[2 * i]) * scale, __uint_as_float(r[2 * i + 1]) * scale);
+      if constexpr (PER == 1) w[32 * half + i] = r[i];
+      else w[16 * half + i] = E::pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
     }
   }
 
@@ -718,9 +751,7 @@ __global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
     // and hands the slot back before it stores. A lane owns one C row: its 64 columns are
     // whole 32-byte sectors, stored straight from registers.
     const uint32_t q = warp & 3u, e = (warp - 4) >> 2;
-    float scale = 1.0f;
-    if (p.ts_a) scale *= *p.ts_a;
-    if (p.ts_b) scale *= *p.ts_b;
+    const SumScale scale(p.ts_a, p.ts_b);
     const uint32_t leader_tempty0 = mapa_shared(bar_tempty, 0);
     uint32_t it = 0;
     bool ok = true;
@@ -755,8 +786,8 @@ __global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty0 + 8 * slot);
-          out[x].set(r[0], 0, scale);
-          out[x].set(r[1], 1, scale);
+          out[x].template set<FMT>(r[0], 0, scale);
+          out[x].template set<FMT>(r[1], 1, scale);
         }
         if (!ok) break;
         if (row0 < p.M) {

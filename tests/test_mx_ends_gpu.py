@@ -3,6 +3,9 @@ forms (mx_check.py).
 
 Tolerances
 - a found tensor scale is one fp32 product, so it is compared for equality.
+- products of integer data with far tensor scales: the sum is exact, the scales' product and its
+  product with the sum round once each (2^-24), a result below the normal numbers once more
+  (2^-150); bf16 adds its half step, 2^-8, or 2^-134 below the normal numbers.
 """
 from __future__ import annotations
 
@@ -94,4 +97,42 @@ def test_norm_in_place_at_odd_pitches(b200, dtype, rows, cols):
             a, b = bx[:, 1:cols + 1].copy_(x), br[:, 1:cols + 1].copy_(r)
             t, k = b200.rms_norm_mx(a, w, b, residual_out=a if over_x else b)
             assert torch.equal(k, h) and torch.equal(t.data, want.data) and torch.equal(t.scales, want.scales)
+    _ok(b200)
+
+
+def _operand(b200, code, byte, fmt, cols, ts):
+    s = torch.tensor([ts], dtype=torch.float32, device="cuda")
+    return b200.MxTensor(torch.from_numpy(X.element_bytes(code, fmt)).cuda(),
+                         torch.from_numpy(X.scale_tiles(byte)).cuda(), fmt, code.shape[0], cols, s)
+
+
+@pytest.mark.parametrize("M", [3, 40, 300])
+@pytest.mark.parametrize("small,ta,tb", [
+    (False, 1.3 * 2.0 ** -100, 1.7 * 2.0 ** -40),  # the scales' product is subnormal, results are not
+    (False, 1.3 * 2.0 ** -90, 1.7 * 2.0 ** -75),   # it rounds to zero, results are subnormal or 0
+    (False, 2.0 ** -126, 2.0 ** -126),
+    (True, 1.3 * 2.0 ** 67, 1.7 * 2.0 ** 66),      # it overflows, results do not
+    (False, 1.3 * 2.0 ** 67, 1.7 * 2.0 ** 66),     # both do, but for sums of zero
+    (False, 1.9 * 2.0 ** 127, 1.9 * 2.0 ** 127),
+    (False, 1.9 * 2.0 ** 127, 1.5 * 2.0 ** -126),
+])
+def test_product_with_far_tensor_scales(b200, M, small, ta, tb):
+    rng = np.random.default_rng(M)
+    N, K = 390, 352
+    (ca, ba), (cb, bb) = (X.random_operand(rng, n, K, "nvfp4", exact=True) for n in (M, N))
+    if small:  # every block scale 2^-9
+        ba[:], bb[:] = 1, 1
+    ca[1], cb[7] = 0, 0  # sums of zero
+    a, b = _operand(b200, ca, ba, "nvfp4", K, ta), _operand(b200, cb, bb, "nvfp4", K, tb)
+    ref = X.values(ca, ba, "nvfp4", K) @ X.values(cb, bb, "nvfp4", K).T
+    ref = ref * np.float64(np.float32(ta)) * np.float64(np.float32(tb))
+    for dtype, half, low in ((torch.float32, 0.0, 0.0), (torch.bfloat16, 2.0 ** -8, 2.0 ** -134)):
+        c = b200.gemm_mx(a, b, out_dtype="f32" if dtype is torch.float32 else "bf16").double().cpu().numpy()
+        top = float(torch.finfo(dtype).max)
+        tol = (half + 2.02 * 2.0 ** -24) * np.abs(ref) + 2.0 ** -150 + low
+        assert not np.isnan(c).any() and bool((c[1] == 0).all()) and bool((c[:, 7] == 0).all())
+        big = np.abs(ref) > top * (1 + 2.0 ** -7)  # certain to round beyond the type
+        assert (np.abs(c[big]) == np.inf).all() and (np.sign(c[big]) == np.sign(ref[big])).all()
+        fits = np.abs(ref) < top * (1 - 2.0 ** -7)
+        assert (np.abs(c - ref)[fits] <= tol[fits]).all()
     _ok(b200)
