@@ -515,11 +515,11 @@ __device__ __forceinline__ float reciprocal_root(float m) {
 //     and normalised as that row with eps times its square, which is the same y;
 //   * h * w below could leave fp32 though y does not (h = 2^60, w = 2^80): h is multiplied by
 //     the factor first. Without this only |y| from 2^120 on overflows.
-// NaN rows stay as they are, rows with an infinity come back with the same sum.
-__device__ __forceinline__ bool far_factor(float rstd) { return !(rstd > 0x1p-8f && rstd < 0x1p10f); }
+// NaN rows stay as they are, rows with an infinity come back with the same sum. Returns the
+// row's factor, 1 where h was multiplied by it, then by `lift` too.
 template <int CH, typename Join>
 __device__ __forceinline__ float rescale_row(float (&v)[CH][16], float ss, float rstd, float inv_cols, float eps,
-                                             Join&& join) {
+                                             float lift, Join&& join) {
   if (ss > 0x1p120f || (ss < 0x1p-90f && eps < 0x1p-90f)) {
     const float f = ss > 1.0f ? 0x1p-80f : 0x1p100f;
     ss = 0.0f;
@@ -537,8 +537,26 @@ __device__ __forceinline__ float rescale_row(float (&v)[CH][16], float ss, float
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[ch][i] *= rstd;
+    for (int i = 0; i < 16; ++i) v[ch][i] *= rstd * lift;
   return 1.0f;
+}
+
+// A row's factor from its sum of squares: 1 / rms and, for NV_FP4, the reciprocal tensor scale
+// `pre`, which may be any number that fp32 holds. Their product has room on both sides (in
+// norm_store it meets a block's reciprocal scale, 2^-9 to 2^9); where it has not, h is
+// multiplied by the row's own part first and by 2^64 or 2^-64 of a far `pre`, so that h * w and
+// what is left of `pre` are ordinary numbers wherever the quantised value is one. h * w that
+// leaves fp32 by it leaves it behind `pre` too.
+template <int FMT, int CH, typename Join>
+__device__ __forceinline__ float row_factor(float (&v)[CH][16], float ss, float inv_cols, float eps, float pre,
+                                            Join&& join) {
+  const float rstd = reciprocal_root(fmaf(ss, inv_cols, eps));
+  const float both = FMT == NV_FP4 ? rstd * pre : rstd;
+  const bool near = rstd > 0x1p-8f && rstd < 0x1p10f && (FMT != NV_FP4 || (both > 0x1p-100f && both < 0x1p100f));
+  if (near) return both;  // the same for all threads of the row
+  if constexpr (FMT != NV_FP4) return rescale_row(v, ss, rstd, inv_cols, eps, 1.0f, join);
+  const float lift = pre >= 0x1p64f ? 0x1p64f : pre <= 0x1p-64f ? 0x1p-64f : 1.0f;
+  return rescale_row(v, ss, rstd, inv_cols, eps, lift, join) * (pre / lift);
 }
 
 // The last part of both kernels: one 16-element chunk at column c of row `row`, of which n
@@ -653,20 +671,19 @@ __global__ void __launch_bounds__(TR < 256 ? 256 : TR) mx_rms_norm_kernel(const 
     __syncthreads();
     ss = sum_of<WARPS>(red + r_in * WARPS);
   }
-  float rstd = reciprocal_root(fmaf(ss, p.inv_cols, p.eps));
-  if (far_factor(rstd))  // all threads of the row see the same sum
-    rstd = rescale_row(v, ss, rstd, p.inv_cols, p.eps, [&](float sum) {
-      if constexpr (WARPS > 1) {
-        const auto row_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + r_in), "n"(TR) : "memory"); };
-        row_sync();
-        if (lane == 0) red[warp] = sum;
-        row_sync();
-        sum = sum_of<WARPS>(red + r_in * WARPS);
-      }
-      return sum;
-    });
+  float pre = 1.0f;
   if constexpr (FMT == NV_FP4)
-    if (p.tensor_scale) rstd *= __frcp_rn(*p.tensor_scale);
+    if (p.tensor_scale) pre = __frcp_rn(*p.tensor_scale);
+  const float rstd = row_factor<FMT>(v, ss, p.inv_cols, p.eps, pre, [&](float sum) {
+    if constexpr (WARPS > 1) {
+      const auto row_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + r_in), "n"(TR) : "memory"); };
+      row_sync();
+      if (lane == 0) red[warp] = sum;
+      row_sync();
+      sum = sum_of<WARPS>(red + r_in * WARPS);
+    }
+    return sum;
+  });
 #pragma unroll
   for (int ch = 0; ch < CH; ++ch) {
     const int c = (ch * TR + t) * 16;
@@ -761,15 +778,12 @@ __global__ void __launch_bounds__(NT, CH == 1 ? 1024 / NT : 1) mx_rms_norm_strea
     // every thread has read the stage: refill it
     if (threadIdx.x == 0 && row + kNormStages * step < p.rows) load_row(row + kNormStages * step, s);
     ss = sum_of<NT / 32>(red[parity]);
-    float rstd = reciprocal_root(fmaf(ss, p.inv_cols, p.eps));
-    if (far_factor(rstd))  // all threads see the same sum
-      rstd = rescale_row(v, ss, rstd, p.inv_cols, p.eps, [&](float sum) {
-        __syncthreads();
-        if (lane == 0) red[parity][warp] = sum;
-        __syncthreads();
-        return sum_of<NT / 32>(red[parity]);
-      });
-    rstd *= pre;
+    const float rstd = row_factor<FMT>(v, ss, p.inv_cols, p.eps, pre, [&](float sum) {
+      __syncthreads();
+      if (lane == 0) red[parity][warp] = sum;
+      __syncthreads();
+      return sum_of<NT / 32>(red[parity]);
+    });
     parity ^= 1u;  // the other buffer: a fast warp's next sum must not overtake a slow one's read
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {

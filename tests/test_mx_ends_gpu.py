@@ -6,6 +6,8 @@ Tolerances
 - products of integer data with far tensor scales: the sum is exact, the scales' product and its
   product with the sum round once each (2^-24), a result below the normal numbers once more
   (2^-150); bf16 adds its half step, 2^-8, or 2^-134 below the normal numbers.
+- the norm: codes of a value within 2^-17 of the exact one (test_mx_gpu.py); the detour of a far
+  factor adds two roundings (2^-24 each), for which the 2^-17 has room.
 """
 from __future__ import annotations
 
@@ -13,6 +15,7 @@ import numpy as np
 import pytest
 
 import mx_check as X
+from test_mx_gpu import _check_norm, _f64, _input, _norm_ref
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -135,4 +138,22 @@ def test_product_with_far_tensor_scales(b200, M, small, ta, tb):
         assert (np.abs(c[big]) == np.inf).all() and (np.sign(c[big]) == np.sign(ref[big])).all()
         fits = np.abs(ref) < top * (1 - 2.0 ** -7)
         assert (np.abs(c - ref)[fits] <= tol[fits]).all()
+    _ok(b200)
+
+
+@pytest.mark.parametrize("rows,cols", [(3, 300), (3, 900), (40, 2000), (601, 4096), (601, 4200), (5, 20001)])
+@pytest.mark.parametrize("ex,ew,et", [(-9, -115, -120), (0, -124, -122), (0, -110, -126), (-60, -100, -108),
+                                      (60, -100, -104), (9, 112, 118), (-60, 100, 104), (60, 110, 112), (0, 0, -30),
+                                      (0, 0, 20)])
+def test_norm_with_far_tensor_scales(b200, rows, cols, ex, ew, et):
+    """The row's factor, the weights or the tensor scale near the ends of fp32, where the value
+    that is quantised is an ordinary one."""
+    x = (_input(cols, rows, cols, "f32") * 2.0 ** ex).to(torch.bfloat16)
+    x[1] = 0
+    w = (1 + 0.2 * torch.randn(cols, generator=torch.Generator().manual_seed(cols))).cuda() * 2.0 ** ew
+    ts = 1.25 * 2.0 ** et
+    t, _ = b200.rms_norm_mx(x, w, eps=0.0, fmt="nvfp4", tensor_scale=torch.tensor([ts], device="cuda"))
+    with np.errstate(invalid="ignore"):
+        y, _ = _norm_ref(_f64(x), _f64(w), None, 0.0)
+    _check_norm(t, np.where(np.isnan(y), 0.0, y), ts)  # a row of zeros stays zero
     _ok(b200)
