@@ -260,10 +260,11 @@ __global__ void __launch_bounds__(256, 1)
   const uint32_t ring = S * Cfg::STAGE;
   const uint32_t bar_off = ring > Cfg::PARTIAL ? ring : Cfg::PARTIAL;
   const uint32_t sBar = base + bar_off;
-  // full[8], empty[8], tfull, done; the TMEM address and the abort flag
+  // full[8], empty[8], tfull, done; the TMEM address, the abort flag, the issued stages
   const uint32_t bar_full = sBar, bar_empty = sBar + 64, bar_tfull = sBar + 128, bar_done = sBar + 136;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + bar_off + 144);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_ptr + bar_off + 148);
+  volatile uint32_t* issued_word = reinterpret_cast<volatile uint32_t*>(base_ptr + bar_off + 152);
 
   const uint32_t warp = __shfl_sync(0xffffffffu, warp_id(), 0), lane = lane_id();
   if (warp == 0 && lane == 0) {
@@ -304,12 +305,10 @@ __global__ void __launch_bounds__(256, 1)
   if (warp == 0) {
     if (elect_one()) {
       uint32_t stage = 0, phase = 0, issued = 0;
-      bool ok = true;
       const uint64_t hint_p = policy_evict_first(), hint_q = policy_evict_last();
       for (uint32_t kb = k0; kb < k1; ++kb) {
         if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1u, p.wait_ns, abort_flag)) {
           fail(ST_PRODUCER_EMPTY);
-          ok = false;
           break;
         }
         const uint32_t g0 = kb * Cfg::GROUPS;
@@ -323,15 +322,7 @@ __global__ void __launch_bounds__(256, 1)
         ++issued;
         if (++stage == S) { stage = 0; phase ^= 1u; }
       }
-      if (!ok || *abort_flag) {
-        // no copy may land after this CTA's shared memory is released
-        for (uint32_t i = issued > S ? issued - S : 0u; i < issued; ++i) {
-          if (!mbar_wait_bounded(bar_full + 8 * (i % S), (i / S) & 1u, p.wait_ns)) {
-            fail(ST_DRAIN);
-            break;
-          }
-        }
-      }
+      *issued_word = issued;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -404,7 +395,19 @@ __global__ void __launch_bounds__(256, 1)
     tmem_dealloc<1>(tmem_base, Cfg::TMEM_COLS);
   }
   if (p.splits > 1) cluster_sync();
-  if (!*abort_flag) {
+  if (*abort_flag) {
+    // No copy may land after this CTA's shared memory is released. Looked at behind every
+    // role's end: a role may give up long after the producer issued its last copy.
+    if (warp == 0 && lane == 0) {
+      const uint32_t issued = *issued_word;
+      for (uint32_t i = issued > S ? issued - S : 0u; i < issued; ++i) {
+        if (!mbar_wait_bounded(bar_full + 8 * (i % S), (i / S) & 1u, p.wait_ns)) {
+          fail(ST_DRAIN);
+          break;
+        }
+      }
+    }
+  } else {
     const SumScale scale(p.ts_p, p.ts_q);
     const uint32_t rows = min(uint32_t(NT), p.nq - q0);
     const uint32_t col = p0 + 4 * lane;

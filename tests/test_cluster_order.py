@@ -63,3 +63,12 @@ def test_cluster_has_started_before_remote_shared_memory():
                 found += 1
                 assert re.search(STARTED, block[:remote.start()]), f"{path.name}: {name}"
     assert found >= 3
+
+
+def test_block_scaled_products_drain_behind_every_role():
+    text = code(CSRC / "mx_gemm.cuh")
+    for name, joined in (("mx_gemm_rows_kernel", "__syncthreads()"), ("mx_gemm_pair_kernel", "cluster_sync()")):
+        block = body(text, re.search(r"__global__[^{]*\b%s\(" % name, text).end())
+        roles_end = block.index(joined, block.index("tmem_wait_ld"))
+        drains = [m.start() for m in re.finditer(r"\(i / S\) & 1u", block)]
+        assert drains and min(drains) > roles_end, name
