@@ -60,6 +60,7 @@ EXPORTS = [
     "b200_mx_dequantize",
     "b200_mx_gemm",
     "b200_mx_rms_norm",
+    "b200_mx_wait_limit",
 ]
 GATHER_MULTICAST, GATHER_PEERS = 1, 2
 MX_FORMATS = {"mxfp8": 0, "mxfp4": 1, "nvfp4": 2}
@@ -181,6 +182,7 @@ def lib():
         L.b200_mx_gemm.argtypes = [C.POINTER(MxDesc), C.POINTER(MxDesc), C.c_void_p, C.c_int32, C.c_int64,
                                    C.c_void_p]
         L.b200_mx_rms_norm.argtypes = [C.POINTER(MxNormArgs), C.POINTER(MxDesc), C.c_void_p]
+        L.b200_mx_wait_limit.argtypes = [C.c_uint64, C.c_int32]
         _LIB = L
     return _LIB
 

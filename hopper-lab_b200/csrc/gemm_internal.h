@@ -67,6 +67,13 @@ int gemm_encode_tiles(CUtensorMap* m, const void* ptr, uint64_t groups, uint64_t
 // Checks of one microscaled operand that need no GPU.
 int mx_validate(const B200MxTensor* t);
 
+// What b200_mx_wait_limit set for this host thread.
+struct MxWaits {
+  uint64_t wait_ns;
+  uint32_t fault_inject;
+};
+const MxWaits& mx_waits();
+
 int gemm_prepare(const B200GemmArgs& a, int sms, int cc_major, uint32_t* status, bool allow_workspace,
                  const GatherSpec* gather, Prepared* out);
 int gemm_launch_prepared(Prepared& pr, cudaStream_t stream);

@@ -13,7 +13,6 @@ namespace {
 
 using namespace b200;
 
-constexpr uint64_t kWaitNs = 1000000000ull;  // 1 s per device wait
 // Block-rows of tiles per group of the pair kernel. Back to back, 8192^3 runs at the power
 // limit, where what is read again from L2 and DRAM costs clock: NV_FP4 231 us with 16, 236
 // with 8, 229 with 32, 250 with 4; MX_FP8 452, 457, 484 and 486.
@@ -149,7 +148,8 @@ int launch_rows(const Call& k) {
   const uint32_t es = uint32_t(elem_size(k.cd));
   p.vec = (reinterpret_cast<uintptr_t>(k.c) % (4 * es)) == 0 && k.ldc % 4 == 0;
   p.status = k.status;
-  p.wait_ns = kWaitNs;
+  p.wait_ns = mx_waits().wait_ns;
+  p.fault_inject = mx_waits().fault_inject;
 
   CUtensorMap tp, tq;
   rc = gemm_encode_2d(&tp, k.b->data, B200_DT_E4M3, p.np, p.row_bytes, uint64_t(k.b->ld), 128, 128);
@@ -212,7 +212,8 @@ int launch_pair(const Call& k) {
   p.align = 32;
   while (bits % p.align) p.align /= 2;
   p.status = k.status;
-  p.wait_ns = kWaitNs;
+  p.wait_ns = mx_waits().wait_ns;
+  p.fault_inject = mx_waits().fault_inject;
 
   CUtensorMap ta, tb, tsa, tsb;
   rc = gemm_encode_2d(&ta, k.a->data, B200_DT_E4M3, p.M, p.row_bytes, uint64_t(k.a->ld), 128, 128);

@@ -154,6 +154,7 @@ struct MxParams {
   uint32_t vec;   // C rows take 4-element stores
   uint32_t* status;
   uint64_t wait_ns;
+  uint32_t fault_inject;  // test hook: 1 = the producer issues no loads, 2 = the MMA warp gives up
 };
 
 // ---------------------------------------------------------------------------------
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(256, 1)
     if (elect_one()) {
       uint32_t stage = 0, phase = 0, issued = 0;
       const uint64_t hint_p = policy_evict_first(), hint_q = policy_evict_last();
-      for (uint32_t kb = k0; kb < k1; ++kb) {
+      for (uint32_t kb = p.fault_inject == 1 ? k1 : k0; kb < k1; ++kb) {
         if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1u, p.wait_ns, abort_flag)) {
           fail(ST_PRODUCER_EMPTY);
           break;
@@ -328,8 +329,9 @@ __global__ void __launch_bounds__(256, 1)
   } else if (warp == 1) {
     if (elect_one()) {
       uint32_t stage = 0, phase = 0;
-      bool ok = true;
-      for (uint32_t kb = k0; kb < k1; ++kb) {
+      bool ok = p.fault_inject != 2;
+      if (!ok) fail(ST_MMA_FULL);
+      for (uint32_t kb = k0; kb < k1 && ok; ++kb) {
         if (!mbar_wait(bar_full + 8 * stage, phase, p.wait_ns, abort_flag)) {
           fail(ST_MMA_FULL);
           ok = false;
@@ -458,6 +460,7 @@ struct MxPairParams {
   uint32_t align;  // of C's rows: 32, 16, 8, 4 or 2 bytes
   uint32_t* status;
   uint64_t wait_ns;
+  uint32_t fault_inject;  // test hook: 1 = the producer issues no loads, 2 = the MMA warp gives up
 };
 
 template <int FMT, int TN>
@@ -662,7 +665,7 @@ __global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
     // =============================== TMA producer ===============================
     if (elect_one()) {
       uint32_t stage = 0, phase = 0, issued = 0;
-      bool ok = true;
+      bool ok = p.fault_inject != 1;
       const uint64_t hint_a = policy_evict_last(), hint_b = policy_evict_first();
       const uint32_t leader_full0 = mapa_shared(bar_full, 0);
       for (uint32_t tile = first_tile; tile < p.num_tiles && ok; tile += tile_stride) {
@@ -701,7 +704,8 @@ __global__ void __launch_bounds__(MxPairCfg<FMT, TN>::THREADS, 1)
     if (rank != 0) {
     } else if (elect_one()) {
       uint32_t stage = 0, phase = 0, it = 0, sf_buf = 0;
-      bool ok = true;
+      bool ok = p.fault_inject != 2;
+      if (!ok) fail(ST_MMA_FULL);
       for (uint32_t tile = first_tile; tile < p.num_tiles && ok; tile += tile_stride, ++it) {
         uint32_t bm, bn;
         tile_to_bmn(tile, p.m_tiles, p.n_tiles, p.group_m, bm, bn);

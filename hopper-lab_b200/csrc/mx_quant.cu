@@ -434,6 +434,7 @@ struct NormParams {
   int32_t wide, wide_weight, weight_f32, stream;
   uint32_t* status;
   uint64_t wait_ns;
+  uint32_t fault_inject;  // test hook: 1 = no loads are issued, 2 = their readers give up
 };
 
 // x + residual is kept unrounded in fp32 for the norm; h is its one rounding. The whole row
@@ -733,7 +734,7 @@ __global__ void __launch_bounds__(NT, CH == 1 ? 1024 / NT : 1) mx_rms_norm_strea
   // behind the ring, only there when h is at an odd pitch
   float* stage = reinterpret_cast<float*>(smem + kNormStages * stage_bytes) + warp * kStageFloats;
   const int64_t first = blockIdx.x, step = gridDim.x;
-  if (threadIdx.x == 0)
+  if (threadIdx.x == 0 && p.fault_inject != 1)
     for (int s = 0; s < kNormStages; ++s)
       if (first + s * step < p.rows) load_row(first + s * step, s);
   float pre = 1.0f;
@@ -742,8 +743,9 @@ __global__ void __launch_bounds__(NT, CH == 1 ? 1024 / NT : 1) mx_rms_norm_strea
 
   int s = 0;
   uint32_t phase = 0, parity = 0;
-  bool ok = true;
-  for (int64_t row = first; row < p.rows; row += step) {
+  bool ok = p.fault_inject != 2;
+  int64_t row = first;
+  for (; row < p.rows && ok; row += step) {
     // all threads wait; a wait that runs out ends this CTA's work (status word)
     ok = mbar_wait_bounded(smem_u32(full + s), phase, p.wait_ns);
     const uint8_t* sx = smem + s * stage_bytes;
@@ -800,11 +802,15 @@ __global__ void __launch_bounds__(NT, CH == 1 ? 1024 / NT : 1) mx_rms_norm_strea
     }
   }
   if (!ok) {
-    // a copy never landed: report it, and wait once more for those in flight before the
-    // shared memory goes away
+    // a copy never landed: report it, and wait once more for those in flight (this row's and the
+    // ones behind it) before the shared memory goes away
     if (threadIdx.x == 0) {
-      if (p.status) atomicOr(p.status, ST_PRODUCER_EMPTY | ST_ABORTED);
-      for (int i = 0; i < kNormStages; ++i) (void)mbar_wait_bounded(smem_u32(full + i), i < s ? phase ^ 1u : phase, p.wait_ns);
+      uint32_t code = ST_PRODUCER_EMPTY | ST_ABORTED;
+      for (int i = 0; i < kNormStages && row + i * step < p.rows; ++i) {
+        const int at = s + i < kNormStages ? s + i : s + i - kNormStages;
+        if (!mbar_wait_bounded(smem_u32(full + at), at < s ? phase ^ 1u : phase, p.wait_ns)) code |= ST_DRAIN;
+      }
+      if (p.status) atomicOr(p.status, code);
     }
     __syncthreads();
   }
@@ -994,6 +1000,10 @@ int norm_f(int dt, const NormParams& p, int sms, int dev, cudaStream_t s) {
 
 namespace b200 {
 
+constexpr uint64_t kDefaultWaitNs = 1000000000ull;  // 1 s per device wait
+static thread_local MxWaits t_waits = {kDefaultWaitNs, 0};
+const MxWaits& mx_waits() { return t_waits; }
+
 // Checks of one microscaled operand that need no GPU.
 int mx_validate(const B200MxTensor* t) {
   if (!t || t->format < B200_MX_FP8 || t->format > B200_NV_FP4 || t->reserved != 0) return B200_ERR_INVALID_ARG;
@@ -1019,6 +1029,12 @@ int b200_mx_layout(int32_t format, int64_t rows, int64_t cols, int64_t* row_byte
   if (rows < 0 || cols < 0 || rows > lim || cols > lim) return B200_ERR_SHAPE;
   if (row_bytes) *row_bytes = mx_row_bytes(format, cols);
   if (scale_bytes) *scale_bytes = mx_scale_bytes(format, rows, cols);
+  return B200_OK;
+}
+
+int b200_mx_wait_limit(uint64_t wait_limit_ns, int32_t fault_inject) {
+  if (fault_inject < 0 || fault_inject > 2) return B200_ERR_INVALID_ARG;
+  b200::t_waits = {wait_limit_ns ? wait_limit_ns : b200::kDefaultWaitNs, uint32_t(fault_inject)};
   return B200_OK;
 }
 
@@ -1109,7 +1125,8 @@ int b200_mx_rms_norm(const B200MxNormArgs* a, const B200MxTensor* q, void* strea
   NormParams p{};
   rc = b200::gemm_device(&dev, &sms, &p.status);
   if (rc != B200_OK) return rc;
-  p.wait_ns = 1000000000ull;  // 1 s per device wait
+  p.wait_ns = mx_waits().wait_ns;
+  p.fault_inject = mx_waits().fault_inject;
   p.x = a->x;
   p.weight = a->weight;
   p.residual = a->residual;

@@ -277,6 +277,13 @@ typedef struct B200MxNormArgs {
 } B200MxNormArgs;
 int b200_mx_rms_norm(const B200MxNormArgs* args, const B200MxTensor* q, void* stream);
 
+/* Bound of each device wait of the b200_mx_* calls that this host thread makes from now on,
+ * 0 = library default (1 s). A wait that runs out ends its kernel's work with what the call
+ * writes undefined and is reported by b200_gemm_status. fault_inject: 0 in production; test
+ * hooks: 1 = the producers of b200_mx_gemm and of the norm's streaming kernel issue no loads,
+ * so the waits must run out; 2 = their consumers give up at once, with loads in flight. */
+int b200_mx_wait_limit(uint64_t wait_limit_ns, int32_t fault_inject);
+
 /* ABI version (B200GEMM_ABI_VERSION). */
 int b200_gemm_abi_version(void);
 

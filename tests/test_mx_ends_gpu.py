@@ -157,3 +157,58 @@ def test_norm_with_far_tensor_scales(b200, rows, cols, ex, ew, et):
         y, _ = _norm_ref(_f64(x), _f64(w), None, 0.0)
     _check_norm(t, np.where(np.isnan(y), 0.0, y), ts)  # a row of zeros stays zero
     _ok(b200)
+
+
+@pytest.fixture
+def waits(b200):
+    yield b200.lib().b200_mx_wait_limit
+    assert b200.lib().b200_mx_wait_limit(0, 0) == 0
+
+
+# rows kernel with and without K splits, and at both ring depths; pairs of every tile width
+@pytest.mark.parametrize("fmt,M,N,K", [("nvfp4", 3, 1000, 8192), ("mxfp8", 20, 3000, 160), ("mxfp4", 100, 30000, 2048),
+                                       ("nvfp4", 600, 900, 512), ("mxfp8", 2500, 2500, 1024),
+                                       ("mxfp4", 4000, 4000, 1056)])
+@pytest.mark.parametrize("hook", [1, 2])
+def test_product_waits_run_out(b200, waits, fmt, M, N, K, hook):
+    """Loads that never come, or an MMA warp that gives up with loads in flight: the kernel ends,
+    the status word says so, and the next call is right."""
+    rng = np.random.default_rng(K)
+    (ca, ba), (cb, bb) = (X.random_operand(rng, n, K, fmt, exact=True) for n in (M, N))
+    a, b = (b200.MxTensor(torch.from_numpy(X.element_bytes(c, fmt)).cuda(), torch.from_numpy(X.scale_tiles(s)).cuda(),
+                          fmt, c.shape[0], K) for c, s in ((ca, ba), (cb, bb)))
+    want = X.values(ca, ba, fmt, K) @ X.values(cb, bb, fmt, K).T
+    c = torch.empty(M, N, device="cuda")
+    for rep in range(3):
+        assert waits(10_000_000, hook) == 0
+        b200.gemm_mx(a, b, c)
+        rc, bits = b200.status()
+        assert rc == b200.ERR_DEVICE_TIMEOUT and bits & 0x80000000, (rc, hex(bits))
+        assert waits(0, 0) == 0
+        c.fill_(float("nan"))
+        b200.gemm_mx(a, b, c)
+        _ok(b200)
+        np.testing.assert_array_equal(_f64(c), want)
+
+
+# column counts that stream: the register kernel, which takes 4096, has no waits
+@pytest.mark.parametrize("cols,residual", [(4112, True), (12000, False), (2056, True), (5008, False)])
+@pytest.mark.parametrize("hook", [1, 2])
+def test_norm_waits_run_out(b200, waits, cols, residual, hook):
+    g = torch.Generator().manual_seed(cols)
+    rows = 1500  # several rounds of the ring
+    x, r = (torch.randn(rows, cols, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    r = r if residual else None
+    w = torch.ones(cols, device="cuda", dtype=torch.bfloat16)
+    want, h = b200.rms_norm_mx(x, w, r)
+    _ok(b200)
+    for rep in range(3):
+        assert waits(10_000_000, hook) == 0
+        b200.rms_norm_mx(x, w, r)
+        rc, bits = b200.status()
+        assert rc == b200.ERR_DEVICE_TIMEOUT and bits & 0x80000000, (rc, hex(bits))
+        assert waits(0, 0) == 0
+        t, k = b200.rms_norm_mx(x, w, r)
+        _ok(b200)
+        assert torch.equal(t.data, want.data) and torch.equal(t.scales, want.scales)
+        assert not residual or torch.equal(k, h)
