@@ -589,6 +589,8 @@ class _On:
             raise ValueError(f"tensors must be on a CUDA device, not {device}")
         self._device = cuda.device(device)
         if stream is not None:
+            if not isinstance(stream, int) and stream.device != device:
+                raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
             stream = cuda.stream(cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
         self._stream = stream
 
