@@ -562,6 +562,13 @@ def _mx_output(name, rows, cols, device):
     return _empty_strided((rows, cols), (ld, 1), dtype=kind[0], device=device), kind[1], ld
 
 
+def _mx_failed(rc, what, out, kept):
+    """Raise for a refused call that was to write `out`, which keeps the scale it had."""
+    if out is not None:
+        out._ts, out._desc.tensor_scale = kept
+    raise B200Error(rc, what)
+
+
 def _mx_out(out, rows, cols, fmt, device, tensor_scale):
     if out is None:
         if fmt not in MX_FORMATS:
@@ -632,13 +639,14 @@ def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=
     rows, cols = x.shape
     if transpose:
         rows, cols = cols, rows
+    kept = None if out is None else (out._ts, out._desc.tensor_scale)
     t = _mx_out(out, rows, cols, fmt, device, tensor_scale)
     find = fmt == "nvfp4" and tensor_scale is None
     if find:
         t._scratch()
     rc = _LIB.b200_mx_quantize(x.data_ptr(), dt, ldx, transpose, find, t._ref, here)
     if rc != OK:
-        raise B200Error(rc, "b200_mx_quantize")
+        _mx_failed(rc, "b200_mx_quantize", out, kept)
     return t
 
 
@@ -725,8 +733,9 @@ def rms_norm_mx(x, weight, residual=None, *, eps: float = 1e-6, fmt: str = "mxfp
             raise TypeError(f"residual and residual_out must be {x.dtype}")
         args = MxNormArgs(dt, wt, x.data_ptr(), weight.data_ptr(), residual.data_ptr(), residual_out.data_ptr(),
                           ldx, ldr, ldh, eps, 0)
+    kept = None if out is None else (out._ts, out._desc.tensor_scale)
     t = _mx_out(out, rows, cols, fmt, device, tensor_scale)
     rc = _LIB.b200_mx_rms_norm(C.byref(args), t._ref, here)
     if rc != OK:
-        raise B200Error(rc, "b200_mx_rms_norm")
+        _mx_failed(rc, "b200_mx_rms_norm", out, kept)
     return t, residual_out

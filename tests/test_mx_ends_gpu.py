@@ -212,3 +212,25 @@ def test_norm_waits_run_out(b200, waits, cols, residual, hook):
         _ok(b200)
         assert torch.equal(t.data, want.data) and torch.equal(t.scales, want.scales)
         assert not residual or torch.equal(k, h)
+
+
+def test_refused_call_leaves_out_as_it_was(b200):
+    """`out` takes a call's tensor scale; a call that is refused must not change what it stands
+    for."""
+    x, w = torch.randn(20, 96, device="cuda"), torch.ones(96, device="cuda")
+    ts = torch.tensor([0.01], device="cuda")
+    found = b200.quantize_mx(x, "nvfp4")
+    given = b200.quantize_mx(x, "nvfp4", tensor_scale=ts)
+    own = b200.MxTensor(given.data.clone(), given.scales.clone(), "nvfp4", 20, 96, ts)
+    flat = torch.randn(1, 96, device="cuda").expand(20, 96)  # rows at one address: refused
+    for t in (found, given, own):
+        before, scale = b200.dequantize_mx(t, out_dtype="f32"), float(t.tensor_scale)
+        for call in (lambda: b200.rms_norm_mx(x, w, eps=-1.0, fmt="nvfp4", out=t),
+                     lambda: b200.rms_norm_mx(flat, w, fmt="nvfp4", out=t, tensor_scale=torch.ones(1, device="cuda")),
+                     lambda: b200.quantize_mx(flat, "nvfp4", out=t),
+                     lambda: b200.quantize_mx(flat, "nvfp4", out=t, tensor_scale=torch.ones(1, device="cuda"))):
+            with pytest.raises(b200.B200Error):
+                call()
+            assert t.tensor_scale is not None and float(t.tensor_scale) == scale
+            assert torch.equal(b200.dequantize_mx(t, out_dtype="f32"), before)
+    _ok(b200)
