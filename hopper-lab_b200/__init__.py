@@ -651,7 +651,8 @@ def quantize_mx(x, fmt: str = "nvfp4", *, transpose: bool = False, tensor_scale=
 
 
 def dequantize_mx(t: MxTensor, out=None, *, out_dtype="bf16", stream=None):
-    """The values a microscaled matrix stands for, rounded once to f16, bf16 or f32."""
+    """The values a microscaled matrix stands for, rounded to f16, bf16 or f32 (behind a tensor
+    scale to fp32 first)."""
     device = t.device
     here = _here(device, stream)
     if here is None:
@@ -671,7 +672,8 @@ def dequantize_mx(t: MxTensor, out=None, *, out_dtype="bf16", stream=None):
 
 def gemm_mx(a: MxTensor, b: MxTensor, c=None, *, out_dtype="bf16", stream=None):
     """C = A . B^T of the values two microscaled matrices stand for (A: M x K, B: N x K,
-    same format), fp32 accumulation, to f16, bf16 or f32. Any row stride of C is accepted."""
+    same format), fp32 accumulation, to f16, bf16 or f32. Any row stride of C is accepted. A
+    device wait that runs out leaves C undefined and shows in :func:`status`."""
     device = a.device
     if a.fmt != b.fmt:
         raise TypeError(f"A and B must have the same format, not {a.fmt} and {b.fmt}")
@@ -696,8 +698,8 @@ def gemm_mx(a: MxTensor, b: MxTensor, c=None, *, out_dtype="bf16", stream=None):
 def rms_norm_mx(x, weight, residual=None, *, eps: float = 1e-6, fmt: str = "mxfp8", tensor_scale=None,
                 out: MxTensor | None = None, residual_out=None, stream=None):
     """RMS norm with the residual's addition, to a microscaled matrix: h = x + residual,
-    out = quantised(h / sqrt(mean(h^2) + eps) * weight). Returns (out, h), h rounded to x's
-    type, or (out, None) without a residual. ``residual_out`` may be ``residual`` or ``x``,
+    out = quantised(h / sqrt(mean(h^2) + eps) * weight), up to 2^-17 of that value. Returns
+    (out, h), h rounded to x's type, or (out, None) without a residual. ``residual_out`` may be ``residual`` or ``x``,
     and overlaps neither otherwise. ``weight`` has x's type or is float32; ``tensor_scale``
     ("nvfp4") is used as given, None stands for 1, which suits normalised rows (block maxima
     from 0.006 to 2688)."""

@@ -251,10 +251,13 @@ int launch_pair(const Call& k) {
 // pair kernel, at the tile width whose waves cost least: a wave of 128-, 192- or 384-wide
 // tiles takes time in the ratio 20 : 26 : 47 (8192^3 in 28, 19 and 10 waves: NV_FP4 241,
 // 220 and 197 us, MX_FP8 553, 416 and 403; 512 x 8192 x 8192 in 2, 2 and 1: 19.6, 25.3 and
-// 22.6 us). Where the pairs' tiles do not fill one wave and K is long, the rows kernel's K
-// splits win: it then has `share` atoms of K per CTA and about 12 atoms' time for joining,
-// against all of K (256 x 2048 x 8192 NV_FP4: 8.3 us with 4 splits, 10.9 in pairs; 1024 x
-// 1024 x 4096, 2 splits of 8 atoms: 8.8 against 7.1).
+// 22.6 us). That ratio is NV_FP4's and serves all formats: MX_FP8's own figures make 20 : 22 :
+// 41, and neither K nor C's type or alignment enters, though an fp32 tile of 384 is drained in
+// two parts and odd rows of C take longer. Where the pairs' tiles do not fill one wave and K is
+// long, the rows kernel's K splits win: it then has `share` atoms of K per CTA and about 12
+// atoms' time for joining, against all of K (256 x 2048 x 8192 NV_FP4: 8.3 us with 4 splits,
+// 10.9 in pairs; 1024 x 1024 x 4096, 2 splits of 8 atoms: 8.8 against 7.1); 12 too is one
+// number for three formats whose atoms differ in cost.
 template <int FMT, int CD>
 int run(const Call& k) {
   const int64_t m = k.a->rows, n = k.b->rows;

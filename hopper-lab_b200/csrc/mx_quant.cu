@@ -1,7 +1,7 @@
 // mx_quant.cu — microscaled quantiser, dequantiser and RMS norm (formats: mx_common.cuh).
 //
 //   quantise     rows of x, or of x transposed, to elements + block scales
-//   dequantise   element * block scale * tensor scale, rounded once to f16 / bf16 / f32
+//   dequantise   element * block scale (exact) * tensor scale in fp32, to f16 / bf16 / f32
 //   RMS norm     h = x + residual; y = h * rsqrt(mean(h^2) + eps) * weight; y quantised
 //
 // All are streaming passes bound by HBM: per element they read and write what the

@@ -248,21 +248,27 @@ int b200_mx_quantize(const void* x, int32_t x_dtype, int64_t ldx, int32_t transp
                      const B200MxTensor* q, void* stream);
 
 /* y (q->rows x q->cols, f16 / bf16 / f32, ldy elements between rows) = the values q
- * stands for, rounded once. */
+ * stands for. element * block scale is exact; a tensor scale rounds it to fp32, and the output
+ * type rounds the result. */
 int b200_mx_dequantize(const B200MxTensor* q, void* y, int32_t y_dtype, int64_t ldy, void* stream);
 
 /* C (a->rows x b->rows) = A . B^T of the values two microscaled matrices of the same
- * format and `cols` stand for, fp32 accumulation, one rounding to c_dtype (B200_DT_F16 |
+ * format and `cols` stand for: fp32 accumulation, the sum times the tensor scales in fp32 (which
+ * may be any normal numbers: their product need not be one), rounded to c_dtype (B200_DT_F16 |
  * B200_DT_BF16 | B200_DT_F32). ldc >= b->rows elements; C is aligned to its element and
- * any ldc is accepted. Waits are bounded as b200_gemm's (b200_gemm_status). */
+ * any ldc is accepted. Waits are bounded (b200_mx_wait_limit) and reported as b200_gemm's
+ * (b200_gemm_status). */
 int b200_mx_gemm(const B200MxTensor* a, const B200MxTensor* b, void* c, int32_t c_dtype, int64_t ldc,
                  void* stream);
 
 /* RMS norm to a microscaled matrix: for each row, h = x + residual (x alone without a
- * residual), y = h / sqrt(mean(h^2) + eps) * weight in fp32, q = quantised y (the tensor
- * scale of a B200_NV_FP4 q is used as given). With a residual, h is also stored, rounded
- * to dtype; h may be x or residual itself (same address and pitch) and overlaps neither
- * otherwise. cols <= B200_MX_NORM_MAX_COLS. */
+ * residual), y = h / sqrt(mean(h^2) + eps) * weight, q = quantised y (the tensor scale of a
+ * B200_NV_FP4 q is used as given: positive and normal). y itself is never formed: scales and
+ * elements are those of a value within 2^-17 of y (relative), so next to a border they may be
+ * the neighbours of what b200_mx_quantize makes of y rounded to fp32. h * weight is held in
+ * fp32: |y| from 2^120 on may overflow. With a residual, h is also stored, rounded to dtype; h
+ * may be x or residual itself (same address and pitch) and overlaps neither otherwise.
+ * cols <= B200_MX_NORM_MAX_COLS. */
 #define B200_MX_NORM_MAX_COLS 32768
 typedef struct B200MxNormArgs {
   int32_t dtype;        /* of x, residual and h: B200_DT_F16 | B200_DT_BF16 | B200_DT_F32 */
